@@ -144,13 +144,19 @@ __device__ __forceinline__ bool bringup_mode(const Params& p, int bits) { return
 // tiles: one 512-byte block for the 128 rows of A and one per 128 rows of B, padded so that
 // the next stage stays 1024-byte aligned.
 constexpr int kScaleBlockBytes = 512;  // 128 rows x 4 K blocks of 32
-__host__ __device__ constexpr int scale_stage_bytes(int bn) { return (kScaleBlockBytes * (1 + bn / 128) + 1023) / 1024 * 1024; }
+// How a kernel's operands are scaled (its MX template argument).
+enum : int { kMxNone = 0, kMx8 = 1, kMx4 = 2 };
+constexpr int kMx4StageElems = 256;  // elements of K in a 128-byte row of 4-bit elements
+// Scale blocks of one stage per 128 rows: 128 bytes of K are 4 blocks of 32 fp8 or 8 of fp4.
+__host__ __device__ constexpr int scale_blocks_per_rows(int mx) { return mx == kMx4 ? 2 : 1; }
+__host__ __device__ constexpr int scale_load_bytes(int bn, int mx) { return mx == kMxNone ? 0 : kScaleBlockBytes * scale_blocks_per_rows(mx) * (1 + bn / 128); }
+__host__ __device__ constexpr int scale_stage_bytes(int bn, int mx) { return (scale_load_bytes(bn, mx) + 1023) / 1024 * 1024; }
 // `am` = rows of A that a stage holds: 128, or 32 / 64 for skinny problems (M <= am), whose
 // stages then spend their bytes on B.  The MMA still reads 128 rows from the stage's start; the
 // rows beyond `am` are whatever follows in shared memory and only reach accumulator rows that no
 // one reads (rows >= M are never loaded from TMEM or stored).
-__host__ __device__ constexpr int stage_bytes(int bn, int cg = 1, bool mx = false, int am = kBM) {
-  return (am + bn / cg) * kRowBytes + (mx ? scale_stage_bytes(bn) : 0);
+__host__ __device__ constexpr int stage_bytes(int bn, int cg = 1, int mx = kMxNone, int am = kBM) {
+  return (am + bn / cg) * kRowBytes + scale_stage_bytes(bn, mx);
 }
 // Barrier block that follows the stage ring (and, for am < 128, the slack that the last stage's
 // 128-row A read runs into): full[16], empty[16], acc_full[2], acc_empty[2], drain, TMEM base
@@ -159,16 +165,16 @@ constexpr int kBarrierBytes = 384;
 // Bytes behind the last stage that the MMA's 128-row read of a short A tile still touches: the
 // read covers 16 KB from the stage's start, i.e. the stage's own B tile first, and only runs past
 // the stage when A and B together are shorter than that (32 rows of A with a 64-column tile).
-__host__ __device__ constexpr int a_overrun_bytes(int bn, int cg = 1, bool mx = false, int am = kBM) {
+__host__ __device__ constexpr int a_overrun_bytes(int bn, int cg = 1, int mx = kMxNone, int am = kBM) {
   return kBM * kRowBytes > stage_bytes(bn, cg, mx, am) ? kBM * kRowBytes - stage_bytes(bn, cg, mx, am) : 0;
 }
-__host__ __device__ constexpr int smem_bytes(int bn, int stages, int cg = 1, bool mx = false, int am = kBM) {
+__host__ __device__ constexpr int smem_bytes(int bn, int stages, int cg = 1, int mx = kMxNone, int am = kBM) {
   return stages * stage_bytes(bn, cg, mx, am) + a_overrun_bytes(bn, cg, mx, am) + kBarrierBytes + 1024;
 }
-// Two accumulators of bn columns; a block-scaled kernel adds two sets of 16 scale columns.
-constexpr int kScaleTmemCols = 16;
-__host__ __device__ constexpr int tmem_columns(int bn, bool mx = false) {  // bn is a power of two
-  return mx ? 512 : (2 * bn < 32 ? 32 : 2 * bn);
+// Two accumulators of bn columns; a block-scaled kernel adds two sets of 16 (fp8) or 24 (fp4) scale columns.
+__host__ __device__ constexpr int scale_tmem_cols(int mx) { return mx == kMx4 ? 24 : 16; }
+__host__ __device__ constexpr int tmem_columns(int bn, int mx = kMxNone) {  // bn is a power of two
+  return mx != kMxNone ? 512 : (2 * bn < 32 ? 32 : 2 * bn);
 }
 
 // Has more than `limit` ns passed since `t0`?  A single reading of the global timer is not
@@ -425,7 +431,7 @@ __device__ __forceinline__ void store_row32(OutT* dst, const float (&x)[32], boo
 // rings in the same shared memory.  In the pair, full[] lives in the leader and counts the
 // bytes of both CTAs' copies; empty[] and acc_full[] exist in both CTAs and the leader's
 // commits arrive on each; acc_empty[] lives in the leader and collects both CTAs' epilogues.
-template <int BN, typename OutT, int CG, bool MX = false, int AM = kBM>
+template <int BN, typename OutT, int CG, int MX = kMxNone, int AM = kBM>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                const __grid_constant__ CUtensorMap tmap_sfa, const __grid_constant__ CUtensorMap tmap_sfb, const Params p) {
@@ -434,18 +440,18 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   static_assert(BN == 32 || BN == 64 || BN == 128 || BN == 256, "unsupported tile width");
   static_assert(CG == 1 || CG == 2, "one CTA or a CTA pair");
   constexpr uint32_t kBRows = BN / CG;  // B rows staged by this CTA
-  static_assert(AM == kBM || (CG == 1 && !MX && (AM == 32 || AM == 64)), "short A stages: one CTA, plain operands, 32 or 64 rows");
+  static_assert(AM == kBM || (CG == 1 && MX == kMxNone && (AM == 32 || AM == 64)), "short A stages: one CTA, plain operands, 32 or 64 rows");
   constexpr uint32_t kABytes = AM * kRowBytes;
   constexpr uint32_t kBBytes = kBRows * kRowBytes;
   constexpr uint32_t kStageBytes = stage_bytes(BN, CG, MX, AM);
-  constexpr uint32_t kLoadBytes = kABytes + kBBytes + (MX ? kScaleBlockBytes * (1 + BN / 128) : 0);  // bytes one CTA copies per stage
+  constexpr uint32_t kLoadBytes = kABytes + kBBytes + scale_load_bytes(BN, MX);  // bytes one CTA copies per stage
   constexpr uint32_t kTmemCols = tmem_columns(BN, MX);
   // Block-scaled tiles of 256 columns keep a single accumulator: two of them would fill the
   // 512 TMEM columns and leave none for the scales (the epilogue then does not overlap the next
   // main loop, which costs less than the shared-memory bound of a 128-column tile).
-  constexpr int kAccBufs = (MX && BN == 256) ? 1 : 2;
-  static_assert(!MX || BN == 128 || BN == 256, "block-scaled tiles are 128 or 256 columns wide");
-  static_assert(!MX || kAccBufs * BN + 2 * kScaleTmemCols <= 512, "accumulators and scales share the 512 columns");
+  constexpr int kAccBufs = (MX != kMxNone && BN == 256) ? 1 : 2;
+  static_assert(MX == kMxNone || BN == 128 || BN == 256, "block-scaled tiles are 128 or 256 columns wide");
+  static_assert(MX == kMxNone || kAccBufs * BN + 2 * scale_tmem_cols(MX) <= 512, "accumulators and scales share the 512 columns");
   constexpr int kTileM = kBM * CG;
 
   extern __shared__ uint8_t smem_raw[];
@@ -547,7 +553,7 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     fence_proxy_async_smem();
     prefetch_tensormap(&tmap_a);
     prefetch_tensormap(&tmap_b);
-    if constexpr (MX) {
+    if constexpr (MX != kMxNone) {
       prefetch_tensormap(&tmap_sfa);
       prefetch_tensormap(&tmap_sfb);
     }
@@ -617,7 +623,10 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           // of its own 128 rows of A and the blocks of all BN columns of B.  K stages beyond the
           // data (split-K padding) carry zero-filled operands, so any scale will do there.
           [[maybe_unused]] const uint32_t sf_dst = b_dst + kBBytes;
-          [[maybe_unused]] const int ks = min(kb0 + kb, p.sf_k_stages - 1);
+          // A 4-bit stage takes two neighbouring blocks per 128 rows in one copy; when the data ends in
+          // the first of them the second is another row group's or out of range (zero), and no MMA reads it.
+          constexpr int kSfBlocks = scale_blocks_per_rows(MX);
+          [[maybe_unused]] const int ks = kSfBlocks == 1 ? min(kb0 + kb, p.sf_k_stages - 1) : kSfBlocks * (kb0 + kb);
           [[maybe_unused]] const int sfa_blk = m_blk * CG + static_cast<int>(cta_rank);
           [[maybe_unused]] const int sfb_blk = n_blk * (BN / 128);
           if (p.debug_mode & 8) {
@@ -626,11 +635,11 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             if (leader) mbar_arrive(full_bar(stage));
           } else if constexpr (CG == 1) {
             if (!b_requested) arm(stage);
-            if constexpr (MX) {
+            if constexpr (MX != kMxNone) {
               tma_load_2d(sf_dst, &tmap_sfa, full_bar(stage), 0, sfa_blk * p.sf_k_stages + ks);
 #pragma unroll
               for (int q = 0; q < BN / 128; ++q) {
-                tma_load_2d(sf_dst + (1 + q) * kScaleBlockBytes, &tmap_sfb, full_bar(stage), 0, (sfb_blk + q) * p.sf_k_stages + ks);
+                tma_load_2d(sf_dst + (1 + q) * kSfBlocks * kScaleBlockBytes, &tmap_sfb, full_bar(stage), 0, (sfb_blk + q) * p.sf_k_stages + ks);
               }
             }
             tma_load_2d(a_dst, &tmap_a, full_bar(stage), k_elem, a_row);
@@ -640,11 +649,11 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             // the byte count of the pair.
             const uint32_t leader_full = map_to_cta(full_bar(stage), 0u);
             if (!b_requested) arm(stage);
-            if constexpr (MX) {
+            if constexpr (MX != kMxNone) {
               tma_load_2d_pair(sf_dst, &tmap_sfa, leader_full, 0, sfa_blk * p.sf_k_stages + ks);
 #pragma unroll
               for (int q = 0; q < BN / 128; ++q) {
-                tma_load_2d_pair(sf_dst + (1 + q) * kScaleBlockBytes, &tmap_sfb, leader_full, 0, (sfb_blk + q) * p.sf_k_stages + ks);
+                tma_load_2d_pair(sf_dst + (1 + q) * kSfBlocks * kScaleBlockBytes, &tmap_sfb, leader_full, 0, (sfb_blk + q) * p.sf_k_stages + ks);
               }
             }
             tma_load_2d_pair(a_dst, &tmap_a, leader_full, k_elem, a_row);
@@ -712,12 +721,16 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             if (lane == 0) stamp(p, 4);
           }
           if (elect_one()) {
-            if constexpr (MX) {
+            if constexpr (MX != kMxNone) {
               // Scales of this stage: shared memory -> TMEM (alternating column sets), then the
               // four block-scaled MMAs; tcgen05 operations of one thread execute in order.
               const uint32_t sf_smem = smem_base + static_cast<uint32_t>(stage) * kStageBytes + kABytes + kBBytes;
-              const uint32_t sf_tmem = tmem_base + static_cast<uint32_t>(kAccBufs * BN) + sf_set * kScaleTmemCols;  // behind the accumulators
-              if (do_mma) umma_mx_stage<CG, BN / 128>(tmem_d, a_lo, a_lo + b_off, desc_hi, idesc, kb != 0 ? 1u : 0u, sf_tmem, smem_desc_lo_scales(sf_smem));
+              const uint32_t sf_tmem = tmem_base + static_cast<uint32_t>(kAccBufs * BN) + sf_set * scale_tmem_cols(MX);  // behind the accumulators
+              if constexpr (MX == kMx4) {
+                const int left = p.K - (w.kb0 + kb) * kMx4StageElems;  // elements of K from this stage on
+                const uint32_t mmas = static_cast<uint32_t>(min(left + 63, kMx4StageElems) >> 6);
+                if (do_mma) umma_mx4_stage<CG, BN / 128>(tmem_d, a_lo, a_lo + b_off, desc_hi, idesc, kb != 0 ? 1u : 0u, sf_tmem, smem_desc_lo_scales(sf_smem), mmas);
+              } else if (do_mma) umma_mx_stage<CG, BN / 128>(tmem_d, a_lo, a_lo + b_off, desc_hi, idesc, kb != 0 ? 1u : 0u, sf_tmem, smem_desc_lo_scales(sf_smem));
             } else {
               if (do_mma) umma_stage<CG>(tmem_d, a_lo, a_lo + b_off, desc_hi, idesc, kb != 0 ? 1u : 0u, mma_kind);
             }

@@ -75,13 +75,13 @@ namespace {
 using b200::make_operand_map;
 
 // Packed block scales as a matrix of 32-bit words: one 512-byte row per [128 rows][4 K blocks]
-// block, copied whole and unswizzled.
-int make_scale_map(CUtensorMap* map, const void* base, uint64_t blocks) {
+// block, copied whole (`per_copy` neighbouring blocks at a time) and unswizzled.
+int make_scale_map(CUtensorMap* map, const void* base, uint64_t blocks, uint32_t per_copy) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (fn == nullptr) return b200::fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   cuuint64_t dims[2] = {gemm::kScaleBlockBytes / 4, blocks};
   cuuint64_t strides[1] = {gemm::kScaleBlockBytes};
-  cuuint32_t box[2] = {gemm::kScaleBlockBytes / 4, 1};
+  cuuint32_t box[2] = {gemm::kScaleBlockBytes / 4, per_copy};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -105,26 +105,31 @@ KernelFn select_kernel_cg(int bn, bool f32) {
 // Short-A variants (skinny M): one CTA per tile, 64- or 128-column tiles.
 template <int AM>
 KernelFn select_kernel_short_a(int bn, bool f32) {
-  if (bn == 64) return f32 ? gemm::gemm_tn_kernel<64, float, 1, false, AM> : gemm::gemm_tn_kernel<64, __nv_bfloat16, 1, false, AM>;
-  if (bn == 128) return f32 ? gemm::gemm_tn_kernel<128, float, 1, false, AM> : gemm::gemm_tn_kernel<128, __nv_bfloat16, 1, false, AM>;
+  if (bn == 64) return f32 ? gemm::gemm_tn_kernel<64, float, 1, gemm::kMxNone, AM> : gemm::gemm_tn_kernel<64, __nv_bfloat16, 1, gemm::kMxNone, AM>;
+  if (bn == 128) return f32 ? gemm::gemm_tn_kernel<128, float, 1, gemm::kMxNone, AM> : gemm::gemm_tn_kernel<128, __nv_bfloat16, 1, gemm::kMxNone, AM>;
   return nullptr;
 }
 
-KernelFn select_kernel(int bn, int dtype_c, int cta_group, bool mx, int am) {
+template <int MX>
+KernelFn select_kernel_mx(int bn, bool f32, int cta_group) {
+  if (cta_group == 2) {
+    if (bn == 256) return f32 ? gemm::gemm_tn_kernel<256, float, 2, MX> : gemm::gemm_tn_kernel<256, __nv_bfloat16, 2, MX>;
+    return f32 ? gemm::gemm_tn_kernel<128, float, 2, MX> : gemm::gemm_tn_kernel<128, __nv_bfloat16, 2, MX>;
+  }
+  if (bn == 256) return f32 ? gemm::gemm_tn_kernel<256, float, 1, MX> : gemm::gemm_tn_kernel<256, __nv_bfloat16, 1, MX>;
+  return f32 ? gemm::gemm_tn_kernel<128, float, 1, MX> : gemm::gemm_tn_kernel<128, __nv_bfloat16, 1, MX>;
+}
+
+KernelFn select_kernel(int bn, int dtype_c, int cta_group, int mx, int am) {
   const bool f32 = dtype_c == B200_F32 || dtype_c == B200_I32;  // 32-bit outputs share the store path
   if (am == 32) return select_kernel_short_a<32>(bn, f32);
   if (am == 64) return select_kernel_short_a<64>(bn, f32);
-  if (mx) {
-    if (cta_group == 2) {
-      if (bn == 256) return f32 ? gemm::gemm_tn_kernel<256, float, 2, true> : gemm::gemm_tn_kernel<256, __nv_bfloat16, 2, true>;
-      return f32 ? gemm::gemm_tn_kernel<128, float, 2, true> : gemm::gemm_tn_kernel<128, __nv_bfloat16, 2, true>;
-    }
-    if (bn == 256) return f32 ? gemm::gemm_tn_kernel<256, float, 1, true> : gemm::gemm_tn_kernel<256, __nv_bfloat16, 1, true>;
-    return f32 ? gemm::gemm_tn_kernel<128, float, 1, true> : gemm::gemm_tn_kernel<128, __nv_bfloat16, 1, true>;
-  }
+  if (mx == gemm::kMx4) return select_kernel_mx<gemm::kMx4>(bn, f32, cta_group);
+  if (mx == gemm::kMx8) return select_kernel_mx<gemm::kMx8>(bn, f32, cta_group);
   return cta_group == 2 ? select_kernel_cg<2>(bn, f32) : select_kernel_cg<1>(bn, f32);
 }
 
+// Bytes per stored element; packed 4-bit operands are stored as bytes of two elements (see stored_k).
 int elt_bytes(int dtype) {
   switch (dtype) {
     case B200_F16:
@@ -135,6 +140,7 @@ int elt_bytes(int dtype) {
     case B200_E4M3_E5M2:
     case B200_MXE4M3:
     case B200_MXE5M2:
+    case B200_MXE2M1:
     case B200_I8: return 1;
     case B200_F32:
     case B200_I32: return 4;
@@ -144,13 +150,20 @@ int elt_bytes(int dtype) {
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
-bool is_mx(int dtype) { return dtype == B200_MXE4M3 || dtype == B200_MXE5M2; }
+int mx_mode(int dtype) {
+  if (dtype == B200_MXE2M1) return gemm::kMx4;
+  return dtype == B200_MXE4M3 || dtype == B200_MXE5M2 ? gemm::kMx8 : gemm::kMxNone;
+}
+
+// Stored elements per row of an operand: K, or K / 2 bytes of two 4-bit elements each.
+int64_t stored_k(int dtype, int64_t K) { return dtype == B200_MXE2M1 ? K / 2 : K; }
 
 bool is_f8(int dtype) { return dtype == B200_E4M3 || dtype == B200_E5M2 || dtype == B200_E5M2_E4M3 || dtype == B200_E4M3_E5M2; }
 
 // tcgen05 instruction descriptor for the plan's operand types and MMA shape.
 uint32_t idesc_for(int dtype_ab, uint32_t umma_m, uint32_t umma_n) {
-  if (is_mx(dtype_ab)) {
+  if (dtype_ab == B200_MXE2M1) return sm100::make_idesc_mx4(umma_m, umma_n);
+  if (mx_mode(dtype_ab) != gemm::kMxNone) {
     const uint32_t fmt = dtype_ab == B200_MXE5M2 ? 1u : 0u;
     return sm100::make_idesc_mx(fmt, fmt, umma_m, umma_n);
   }
@@ -168,6 +181,7 @@ uint32_t idesc_for(int dtype_ab, uint32_t umma_m, uint32_t umma_n) {
 
 int mma_kind_for(int dtype_ab) { return dtype_ab == B200_I8 ? sm100::kKindI8 : (is_f8(dtype_ab) ? sm100::kKindF8 : sm100::kKindF16); }
 
+constexpr int kScaleBlockK = 128;    // elements of K that one 512-byte scale block covers
 constexpr int kMaxSmemOptin = 232448;  // 227 KB: the sm_100 per-block opt-in limit
 constexpr int kDefaultSms = 148;
 
@@ -253,7 +267,7 @@ struct b200_gemm_plan {
   int bn = 0;
   int cg = 1;         // CTAs per MMA: 1, or 2 for a CTA pair (cluster of two)
   int am = gemm::kBM; // rows of A per stage: 128, or 32 / 64 for skinny M (see gemm::stage_bytes)
-  bool mx = false;    // block-scaled 8-bit floats: scales come from b200_gemm_plan_set_mx_scales
+  int mx = gemm::kMxNone;  // block-scaled operands: scales come from b200_gemm_plan_set_mx_scales
   const void* sfa = nullptr;
   const void* sfb = nullptr;
   CUtensorMap map_sfa = {}, map_sfb = {};  // all zero (never dereferenced) unless mx
@@ -345,9 +359,9 @@ void plan_tail_split(b200_gemm_plan* plan) {
   // One round, one part per CTA (skinny problems: a few column tiles, a long K): the parts of a
   // tile form a cluster and exchange through its shared memory.  The parking area (a 128 x BN
   // fp32 tile) must fit in the stage ring.  reserved[1] bit 2 keeps the exchange in the workspace.
-  if (plan->cg == 1 && !plan->mx && plan->cluster_exchange_ok && (plan->desc.reserved[1] & 4) == 0 && tail == tiles &&
+  if (plan->cg == 1 && plan->mx == gemm::kMxNone && plan->cluster_exchange_ok && (plan->desc.reserved[1] & 4) == 0 && tail == tiles &&
       tiles * parts <= units &&
-      static_cast<int64_t>(plan->stages) * gemm::stage_bytes(plan->bn, 1, false, plan->am) >= static_cast<int64_t>(gemm::kBM) * plan->bn * 4) {
+      static_cast<int64_t>(plan->stages) * gemm::stage_bytes(plan->bn, 1, gemm::kMxNone, plan->am) >= static_cast<int64_t>(gemm::kBM) * plan->bn * 4) {
     plan->cluster_exchange = true;
     return;  // no flags, no partial tiles in global memory
   }
@@ -476,7 +490,7 @@ int launch(b200_gemm_plan* plan, const void* A, const void* B, void* C, const fl
   const b200_gemm_desc& d = plan->desc;
   B200_REQUIRE(d.dtype_c != B200_I32 || (scale_a == nullptr && scale_b == nullptr),
                "gemm_run: i32 output carries the integer sums unchanged; scales need f32 or bf16 output");
-  B200_REQUIRE(!plan->mx || (plan->sfa != nullptr && plan->sfb != nullptr),
+  B200_REQUIRE(plan->mx == gemm::kMxNone || (plan->sfa != nullptr && plan->sfb != nullptr),
                "gemm_run: a block-scaled plan needs its scales first (b200_gemm_plan_set_mx_scales)");
   int ia = -1, ib = -1;
   for (int i = 0; i < b200_gemm_plan::kMapSlots; ++i) {
@@ -486,7 +500,7 @@ int launch(b200_gemm_plan* plan, const void* A, const void* B, void* C, const fl
   if (ia < 0) {
     ia = plan->map_a_next;
     plan->map_a_ptr[ia] = nullptr;
-    int rc = make_operand_map(&plan->map_a[ia], A, d.dtype_ab, static_cast<uint64_t>(d.M), static_cast<uint64_t>(d.K), static_cast<uint32_t>(plan->am));  // per CTA
+    int rc = make_operand_map(&plan->map_a[ia], A, d.dtype_ab, static_cast<uint64_t>(d.M), static_cast<uint64_t>(stored_k(d.dtype_ab, d.K)), static_cast<uint32_t>(plan->am));  // per CTA
     if (rc != B200_OK) return rc;
     plan->map_a_ptr[ia] = A;
     plan->map_a_next = (ia + 1) % b200_gemm_plan::kMapSlots;
@@ -497,7 +511,7 @@ int launch(b200_gemm_plan* plan, const void* A, const void* B, void* C, const fl
     if (direct_b(plan)) {
       plan->map_b[ib] = plan->map_a[ia];  // never dereferenced: packed B is streamed with 1-D bulk copies
     } else {
-      int rc = make_operand_map(&plan->map_b[ib], B, d.dtype_ab, static_cast<uint64_t>(d.N), static_cast<uint64_t>(d.K),
+      int rc = make_operand_map(&plan->map_b[ib], B, d.dtype_ab, static_cast<uint64_t>(d.N), static_cast<uint64_t>(stored_k(d.dtype_ab, d.K)),
                                 static_cast<uint32_t>(plan->bn / plan->cg));
       if (rc != B200_OK) return rc;
     }
@@ -513,7 +527,7 @@ int launch(b200_gemm_plan* plan, const void* A, const void* B, void* C, const fl
   p.n_blocks = plan->n_blocks;
   p.num_tiles = plan->m_blocks * plan->n_blocks;
   p.num_kb = plan->num_kb;
-  p.kb_elems = plan->kb_elems;
+  p.kb_elems = gemm::kRowBytes / plan->eb_ab;  // in stored elements: the step of the loads' inner coordinate
   p.split_k = plan->split_k;
   p.stages = plan->stages;
   p.raster_group = plan->raster_group;
@@ -526,7 +540,7 @@ int launch(b200_gemm_plan* plan, const void* A, const void* B, void* C, const fl
   p.scale_a = scale_a;
   p.scale_b = scale_b;
   p.C = C;
-  p.sf_k_stages = ceil_div(d.K, gemm::kRowBytes);
+  p.sf_k_stages = ceil_div(d.K, kScaleBlockK);
   p.b_packed = direct_b(plan) ? B : nullptr;
   p.workspace = static_cast<float*>(workspace);
   p.status = plan->status;
@@ -633,13 +647,14 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
                (long long)d.M, (long long)d.N, (long long)d.K);
   B200_REQUIRE(d.M < (1ll << 31) - 256 && d.N < (1ll << 31) - 256 && d.K < (1ll << 31) - 256,
                "gemm_plan_create: each of M, N, K must be below 2^31");
-  const bool mx = is_mx(d.dtype_ab);
-  B200_REQUIRE(d.dtype_ab == B200_F16 || d.dtype_ab == B200_BF16 || is_f8(d.dtype_ab) || d.dtype_ab == B200_I8 || mx,
-               "gemm_plan_create: dtype_ab=%d is not f16, bf16, e4m3, e5m2 (or a mix of the two), i8 or a block-scaled fp8", d.dtype_ab);
-  if (mx) {
+  const int mx = mx_mode(d.dtype_ab);
+  B200_REQUIRE(d.dtype_ab == B200_F16 || d.dtype_ab == B200_BF16 || is_f8(d.dtype_ab) || d.dtype_ab == B200_I8 || mx != gemm::kMxNone,
+               "gemm_plan_create: dtype_ab=%d is not f16, bf16, e4m3, e5m2 (or a mix of the two), i8 or a block-scaled fp8 or fp4", d.dtype_ab);
+  if (mx != gemm::kMxNone) {
     B200_REQUIRE(d.K % 32 == 0, "gemm_plan_create: block-scaled inputs need K %% 32 == 0 (one scale per 32 elements), got K=%lld", (long long)d.K);
     B200_REQUIRE(d.b_layout == B200_B_ROW_MAJOR_NK, "gemm_plan_create: block-scaled inputs take row-major B");
     B200_REQUIRE(d.tile_n == 0 || d.tile_n == 128 || d.tile_n == 256, "gemm_plan_create: block-scaled inputs use tile_n=128 or 256 (got %d)", d.tile_n);
+    B200_REQUIRE(mx != gemm::kMx4 || d.split_k <= 1, "gemm_plan_create: 4-bit inputs do not split K through a workspace (split_k=%d)", d.split_k);
   }
   B200_REQUIRE(d.dtype_c == B200_F32 || d.dtype_c == B200_BF16 || d.dtype_c == B200_I32,
                "gemm_plan_create: dtype_c=%d is not f32, bf16 or i32", d.dtype_c);
@@ -653,8 +668,8 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
   B200_REQUIRE(d.bias_axis == B200_BIAS_AXIS_N || d.bias_axis == B200_BIAS_AXIS_M, "gemm_plan_create: bad bias_axis %d", d.bias_axis);
   const int eb = elt_bytes(d.dtype_ab);
   // TMA needs 16-byte multiples for the row pitch of A and B.
-  B200_REQUIRE((d.K * eb) % 16 == 0, "gemm_plan_create: K=%lld gives a %lld-byte row pitch; it must be a multiple of 16 bytes",
-               (long long)d.K, (long long)(d.K * eb));
+  B200_REQUIRE((stored_k(d.dtype_ab, d.K) * eb) % 16 == 0, "gemm_plan_create: K=%lld gives a %lld-byte row pitch; it must be a multiple of 16 bytes",
+               (long long)d.K, (long long)(stored_k(d.dtype_ab, d.K) * eb));
   if (d.b_layout == B200_B_REF_PRESHUFFLED) {
     // Preconditions of the reference's shuffle_weight (kittens_helpers.py:107-108).
     B200_REQUIRE(d.N % 16 == 0 && d.K % 32 == 0, "gemm_plan_create: preshuffled B needs N %% 16 == 0 and K %% 32 == 0");
@@ -663,7 +678,7 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
                "gemm_plan_create: tile_m=%d unsupported (128, or 256 for a CTA pair)", d.tile_m);
   B200_REQUIRE(d.tile_n == 0 || d.tile_n == 32 || d.tile_n == 64 || d.tile_n == 128 || d.tile_n == 256,
                "gemm_plan_create: tile_n=%d unsupported (32, 64, 128, 256)", d.tile_n);
-  const int kb_elems = gemm::kRowBytes / eb;
+  const int kb_elems = mx == gemm::kMx4 ? gemm::kMx4StageElems : gemm::kRowBytes / eb;
   B200_REQUIRE(d.tile_k == 0 || d.tile_k == kb_elems, "gemm_plan_create: tile_k=%d unsupported (%d for this dtype)", d.tile_k, kb_elems);
   B200_REQUIRE(d.cta_group >= 0 && d.cta_group <= 2, "gemm_plan_create: cta_group=%d unsupported (1 or 2)", d.cta_group);
   B200_REQUIRE(!(d.cta_group == 2 && d.tile_m == gemm::kBM) && !(d.cta_group == 1 && d.tile_m == 2 * gemm::kBM),
@@ -698,7 +713,7 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
   const bool short_k = k_blocks <= 16;
   if (cg == 0) {
     cg = (d.b_layout == B200_B_ROW_MAJOR_NK && d.M >= 2 * gemm::kBM && d.tile_n != 32) ? 2 : 1;
-    if (cg == 2 && short_k && !mx && d.tile_n == 0 &&
+    if (cg == 2 && short_k && mx == gemm::kMxNone && d.tile_n == 0 &&
         static_cast<int64_t>(ceil_div(d.M, gemm::kBM)) * ceil_div(d.N, 32) <= kDefaultSms) {  // 128 x 32 tiles still fit one round
       cg = 1;
     }
@@ -708,7 +723,7 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
     // in one round on more than half of the SMs, up to 64 K blocks (2048^3: 16.3 against 17.0 us;
     // at 128 K blocks the pair's deeper ring and halved B traffic win: 512 x 8192 x 8192 56 against 74 us).
     const int64_t wide_tiles = static_cast<int64_t>(ceil_div(d.M, gemm::kBM)) * ceil_div(d.N, 256);
-    if (cg == 2 && !mx && (k_blocks <= 8 || (k_blocks <= 64 && wide_tiles > kDefaultSms / 2 && wide_tiles <= kDefaultSms))) cg = 1;
+    if (cg == 2 && mx == gemm::kMxNone && (k_blocks <= 8 || (k_blocks <= 64 && wide_tiles > kDefaultSms / 2 && wide_tiles <= kDefaultSms))) cg = 1;
   }
   plan->cg = cg;
   plan->mx = mx;
@@ -717,7 +732,7 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
   // Tile width: the widest tile whose tile count still fills the machine; wide tiles halve the
   // shared-memory traffic per flop, narrow ones keep more SMs busy on small problems.
   int bn = d.tile_n;
-  if (bn == 0 && mx) {
+  if (bn == 0 && mx != gemm::kMxNone) {
     // 256 columns unless that leaves SMs without a tile: a 128-column tile is bound by shared-memory reads.
     bn = (static_cast<int64_t>(plan->m_blocks) * ceil_div(d.N, 256) >= kDefaultSms / cg) ? 256 : 128;
   }
@@ -767,7 +782,7 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
   plan->n_blocks = ceil_div(d.N, bn);
 
   int split = d.split_k <= 1 ? 1 : d.split_k;
-  if (d.split_k == -1 && d.dtype_ab != B200_I8) {  // integer sums never split
+  if (d.split_k == -1 && d.dtype_ab != B200_I8 && mx != gemm::kMx4) {  // integer sums and 4-bit operands never split
     // Skinny problems: too few tiles to occupy the SMs, so cut K until they do, keeping at
     // least four K blocks per partition.
     const int64_t tiles = static_cast<int64_t>(plan->m_blocks) * plan->n_blocks;
@@ -782,7 +797,7 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
   // ring holds more of B, the operand that such a problem streams from HBM.  tile_m = 128
   // asks for full A stages.
   int am = gemm::kBM;
-  if (cg == 1 && !mx && d.tile_m == 0 && d.M <= 64 && (bn == 64 || bn == 128)) am = d.M <= 32 ? 32 : 64;
+  if (cg == 1 && mx == gemm::kMxNone && d.tile_m == 0 && d.M <= 64 && (bn == 64 || bn == 128)) am = d.M <= 32 ? 32 : 64;
   plan->am = am;
   // Full-A stages never profit from more than 8 slots.  Short-A stages belong to problems that
   // stream B from HBM, and a stream of 16 KB copies is fastest with about 100 KB per SM on request
@@ -811,7 +826,7 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
   if (d.raster_group > 0) {
     plan->raster_group = d.raster_group;
   } else {
-    const int64_t block_bytes = static_cast<int64_t>(gemm::kBM) * cg * d.K * eb;
+    const int64_t block_bytes = static_cast<int64_t>(gemm::kBM) * cg * stored_k(d.dtype_ab, d.K) * eb;
     int64_t g = (int64_t{32} << 20) / (block_bytes > 0 ? block_bytes : 1);
     if (g > plan->m_blocks) g = plan->m_blocks;
     plan->raster_group = g < 1 ? 1 : static_cast<int>(g);
@@ -889,7 +904,7 @@ int b200_gemm_debug_timeline(b200_gemm_plan* plan, void* device_buffer) {
 int b200_mx_scales_bytes(int64_t rows, int64_t K, size_t* bytes) {
   B200_REQUIRE(bytes != nullptr, "mx_scales_bytes: bytes is NULL");
   B200_REQUIRE(rows >= 1 && K >= 32 && K % 32 == 0, "mx_scales_bytes: rows must be >= 1 and K a positive multiple of 32");
-  *bytes = static_cast<size_t>(ceil_div(rows, 128)) * ceil_div(K, gemm::kRowBytes) * gemm::kScaleBlockBytes;
+  *bytes = static_cast<size_t>(ceil_div(rows, 128)) * ceil_div(K, kScaleBlockK) * gemm::kScaleBlockBytes;
   return B200_OK;
 }
 
@@ -897,7 +912,7 @@ int b200_pack_mx_scales(const void* scales_in, void* scales_packed, int64_t rows
   B200_REQUIRE(scales_in != nullptr && scales_packed != nullptr, "pack_mx_scales: NULL argument");
   B200_REQUIRE(rows >= 1 && K >= 32 && K % 32 == 0, "pack_mx_scales: rows must be >= 1 and K a positive multiple of 32");
   B200_REQUIRE((reinterpret_cast<uintptr_t>(scales_packed) & 15u) == 0, "pack_mx_scales: output must be 16-byte aligned");
-  const long long row_blocks = ceil_div(rows, 128), k_stages = ceil_div(K, gemm::kRowBytes);
+  const long long row_blocks = ceil_div(rows, 128), k_stages = ceil_div(K, kScaleBlockK);
   long long blocks = (row_blocks * k_stages * gemm::kScaleBlockBytes + 255) / 256;
   if (blocks > 148 * 16) blocks = 148 * 16;
   pack_mx_scales_kernel<<<static_cast<int>(blocks), 256, 0, b200::as_stream(stream)>>>(
@@ -909,14 +924,15 @@ int b200_pack_mx_scales(const void* scales_in, void* scales_packed, int64_t rows
 
 int b200_gemm_plan_set_mx_scales(b200_gemm_plan* plan, const void* scales_a_packed, const void* scales_b_packed) {
   B200_REQUIRE(plan != nullptr, "gemm_plan_set_mx_scales: plan is NULL");
-  B200_REQUIRE(plan->mx, "gemm_plan_set_mx_scales: the plan's dtype_ab is not block-scaled");
+  B200_REQUIRE(plan->mx != gemm::kMxNone, "gemm_plan_set_mx_scales: the plan's dtype_ab is not block-scaled");
   B200_REQUIRE(scales_a_packed != nullptr && scales_b_packed != nullptr, "gemm_plan_set_mx_scales: NULL scales");
   B200_REQUIRE(((reinterpret_cast<uintptr_t>(scales_a_packed) | reinterpret_cast<uintptr_t>(scales_b_packed)) & 15u) == 0,
                "gemm_plan_set_mx_scales: packed scales must be 16-byte aligned");
-  const uint64_t k_stages = static_cast<uint64_t>(ceil_div(plan->desc.K, gemm::kRowBytes));
-  int rc = make_scale_map(&plan->map_sfa, scales_a_packed, static_cast<uint64_t>(ceil_div(plan->desc.M, 128)) * k_stages);
+  const uint64_t k_stages = static_cast<uint64_t>(ceil_div(plan->desc.K, kScaleBlockK));
+  const uint32_t per_copy = static_cast<uint32_t>(gemm::scale_blocks_per_rows(plan->mx));
+  int rc = make_scale_map(&plan->map_sfa, scales_a_packed, static_cast<uint64_t>(ceil_div(plan->desc.M, 128)) * k_stages, per_copy);
   if (rc != B200_OK) return rc;
-  rc = make_scale_map(&plan->map_sfb, scales_b_packed, static_cast<uint64_t>(ceil_div(plan->desc.N, 128)) * k_stages);
+  rc = make_scale_map(&plan->map_sfb, scales_b_packed, static_cast<uint64_t>(ceil_div(plan->desc.N, 128)) * k_stages, per_copy);
   if (rc != B200_OK) return rc;
   plan->sfa = scales_a_packed;
   plan->sfb = scales_b_packed;

@@ -1,0 +1,301 @@
+// Block-scaled 4-bit floats on the device: values -> E2M1 codes and E8M0 scales, and back.
+//
+// A block is 32 consecutive values of a row.  With a = max |x| over the block, the shared exponent
+// is e = floor(log2 a) - 2 (2 is the exponent of E2M1's largest magnitude, 6 = 1.5 * 2^2), clamped
+// to [-127, 127]; the scale byte is e + 127 and the codes are x * 2^-e rounded to nearest even with
+// magnitudes above 6 saturating.  A block of zeros has scale byte 127.  A block that holds a NaN or
+// an infinity has scale byte 255 (E8M0's NaN): all 32 values then read as NaN, here and in the
+// tensor core.  All of it is exact in fp32 but for the one rounding to E2M1: a product with a power
+// of two only rounds where the result is below 2^-126, and that is code 0 either way.
+//
+// The scales are written in the order the product streams them (blocks of [128 rows][4 K blocks],
+// row r of a block at byte (r % 32) * 16 + (r / 32) * 4; see pack_mx_scales_kernel), so that no
+// second pass over them is needed.
+//
+// Both kernels are bound by DRAM: a lane moves 8 values (16 or 32 bytes, one vector access) and 4
+// lanes share a block, so a warp's accesses are contiguous and the block maximum is two shuffles.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp4.h>
+
+#include "common.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPerLane = 8;               // values per lane and step
+constexpr int kChunk = 32 * kPerLane;     // values per warp and step: 8 blocks of 32, 2 scale words
+constexpr int kSteps = 4;                 // chunks per warp, loads of all of them in flight together
+constexpr int kScaleBlockBytes = 512;
+
+// 8 consecutive values as raw 32-bit words.
+template <typename T>
+struct Raw {
+  uint32_t w[kPerLane * sizeof(T) / 4];
+};
+
+template <typename T>
+__device__ __forceinline__ float value(const Raw<T>& r, int i);
+template <>
+__device__ __forceinline__ float value<float>(const Raw<float>& r, int i) { return __uint_as_float(r.w[i]); }
+template <>
+__device__ __forceinline__ float value<__nv_bfloat16>(const Raw<__nv_bfloat16>& r, int i) {
+  return __uint_as_float((i & 1) ? (r.w[i >> 1] & 0xFFFF0000u) : (r.w[i >> 1] << 16));
+}
+template <>
+__device__ __forceinline__ float value<__half>(const Raw<__half>& r, int i) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>((i & 1) ? (r.w[i >> 1] >> 16) : (r.w[i >> 1] & 0xFFFFu))));
+}
+
+template <typename T, bool kVec>
+__device__ __forceinline__ Raw<T> load8(const T* p) {
+  Raw<T> r;
+  if constexpr (kVec) {
+#pragma unroll
+    for (int j = 0; j < static_cast<int>(sizeof(r.w) / 16); ++j) {
+      const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p) + j);
+      r.w[4 * j] = v.x;
+      r.w[4 * j + 1] = v.y;
+      r.w[4 * j + 2] = v.z;
+      r.w[4 * j + 3] = v.w;
+    }
+  } else {
+    T v[kPerLane];
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) v[i] = p[i];
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) r.w[i] = __float_as_uint(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPerLane / 2; ++i) {
+        r.w[i] = static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(&v[2 * i])) |
+                 (static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(&v[2 * i + 1])) << 16);
+      }
+    }
+  }
+  return r;
+}
+
+// Two values -> one byte, `lo` in the low nibble (round to nearest even, saturating at 6).
+__device__ __forceinline__ uint32_t e2m1_pair(float lo, float hi) {
+  return static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(make_float2(lo, hi), __NV_E2M1, cudaRoundNearest));
+}
+
+// Position of the 4-byte scale word of (row, 128-element K group `kg`) in the packed scales.
+__device__ __forceinline__ size_t scale_word(int64_t row, int64_t kg, int64_t k_groups) {
+  const int r = static_cast<int>(row & 127);
+  return static_cast<size_t>((row >> 7) * k_groups + kg) * kScaleBlockBytes + static_cast<size_t>((r & 31) * 16 + (r >> 5) * 4);
+}
+
+// `rows_padded`: rows rounded up to 128; the rows behind the last only get scale bytes of 127, so
+// that every byte of the packed scales is defined.
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kThreads) quantize_mx4_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ scales,
+                                                                int64_t rows, int64_t rows_padded, int64_t K, int64_t row_stride,
+                                                                int64_t chunks) {
+  const int lane = threadIdx.x & 31;
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int64_t k_groups = (K + 127) / 128;
+  const int64_t total = rows_padded * chunks;
+  Raw<T> raw[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int64_t item = warp * kSteps + s;
+    const int64_t row = item / chunks;
+    const int64_t k = (item - row * chunks) * kChunk + lane * kPerLane;
+    if (item < total && row < rows && k < K) {
+      raw[s] = load8<T, kVec>(x + row * row_stride + k);
+    } else {
+#pragma unroll
+      for (int j = 0; j < static_cast<int>(sizeof(raw[s].w) / 4); ++j) raw[s].w[j] = 0u;
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int64_t item = warp * kSteps + s;
+    if (item >= total) break;  // warp-uniform
+    const int64_t row = item / chunks;
+    const int64_t chunk = item - row * chunks;
+    const int64_t k = chunk * kChunk + lane * kPerLane;
+    float v[kPerLane];
+    uint32_t amax = 0u;  // magnitudes compare as integers; infinities and NaN come out largest
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      v[i] = value<T>(raw[s], i);
+      amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    }
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const uint32_t field = amax >> 23;  // biased exponent of the maximum; 0 below 2^-126
+    uint32_t byte = field > 2u ? field - 2u : 0u;
+    if (amax == 0u) byte = 127u;
+    const bool bad = field == 255u;
+    if (bad) byte = 255u;
+    const float inv = bad ? 0.0f : __uint_as_float((254u - byte) << 23);
+    uint32_t codes = 0u;
+    if (!bad) {
+#pragma unroll
+      for (int i = 0; i < kPerLane / 2; ++i) codes |= e2m1_pair(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
+    }
+    if (row < rows && k < K) *reinterpret_cast<uint32_t*>(q + (row * K + k) / 2) = codes;
+    // Four blocks of 32 share a scale word: lanes 0 and 16 collect theirs.
+    uint32_t word = byte << (8 * ((lane >> 2) & 3));
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    const int64_t kg = chunk * 2 + (lane >> 4);
+    if ((lane & 15) == 0 && kg < k_groups) *reinterpret_cast<uint32_t*>(scales + scale_word(row, kg, k_groups)) = word;
+  }
+}
+
+// Rounding into the output type; for bf16 and fp32 it never rounds (two significant bits, and the
+// smallest value, 2^-128, is a bf16 subnormal).
+__device__ __forceinline__ void store8(float* p, const float (&v)[kPerLane]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[kPerLane]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store8(__half* p, const float (&v)[kPerLane]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) dequantize_mx4_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales, T* __restrict__ out,
+                                                                  int64_t rows, int64_t K, int64_t chunks) {
+  const int lane = threadIdx.x & 31;
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int64_t k_groups = (K + 127) / 128;
+  const int64_t total = rows * chunks;
+  uint32_t codes[kSteps], byte[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int64_t item = warp * kSteps + s;
+    const int64_t row = item / chunks;
+    const int64_t k = (item - row * chunks) * kChunk + lane * kPerLane;
+    codes[s] = byte[s] = 0u;
+    if (item < total && k < K) {
+      codes[s] = __ldcs(reinterpret_cast<const uint32_t*>(q + (row * K + k) / 2));
+      byte[s] = __ldg(scales + scale_word(row, k >> 7, k_groups) + ((k >> 5) & 3));
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int64_t item = warp * kSteps + s;
+    const int64_t row = item / chunks;
+    const int64_t k = (item - row * chunks) * kChunk + lane * kPerLane;
+    if (item >= total || k >= K) continue;
+    // 2^(byte - 127): below 2^-126 a subnormal, 255 is NaN
+    const float scale = byte[s] == 255u ? __uint_as_float(0x7FC00000u) : (byte[s] == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte[s] << 23));
+    float v[kPerLane];
+#pragma unroll
+    for (int i = 0; i < kPerLane / 2; ++i) {
+      const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>((codes[s] >> (8 * i)) & 0xFFu), __NV_E2M1);
+      const float2 f = __half22float2(__half2(h));
+      v[2 * i] = f.x * scale;
+      v[2 * i + 1] = f.y * scale;
+    }
+    store8(out + row * K + k, v);
+  }
+}
+
+int check_shape(const char* who, int64_t rows, int64_t K, int dtype_q) {
+  B200_REQUIRE(dtype_q == B200_MXE2M1, "%s: dtype_q=%d is not the block-scaled fp4 type", who, dtype_q);
+  B200_REQUIRE(rows >= 1 && K >= 32 && K % 32 == 0, "%s: rows must be >= 1 and K a positive multiple of 32 (got %lld, %lld)", who, (long long)rows, (long long)K);
+  B200_REQUIRE(rows < (1ll << 31) - 256 && K < (1ll << 31) - 256, "%s: rows and K must be below 2^31", who);
+  return B200_OK;
+}
+
+// One warp per kSteps chunks.
+int grid_for(const char* who, int64_t rows, int64_t chunks, unsigned* grid) {
+  const int64_t per_cta = static_cast<int64_t>(kSteps) * (kThreads / 32);
+  const int64_t ctas = (rows * chunks + per_cta - 1) / per_cta;
+  B200_REQUIRE(ctas < (1ll << 31), "%s: %lld x %lld chunks of 256 values are more than one launch covers", who, (long long)rows, (long long)chunks);
+  *grid = static_cast<unsigned>(ctas);
+  return B200_OK;
+}
+
+template <typename T>
+int launch_quantize(const void* x, void* q, void* scales, int64_t rows, int64_t K, int64_t row_stride, cudaStream_t stream) {
+  const int64_t chunks = (K + kChunk - 1) / kChunk;
+  const int64_t padded = (rows + 127) / 128 * 128;
+  unsigned grid = 0;
+  const int rc = grid_for("quantize_mx", padded, chunks, &grid);
+  if (rc != B200_OK) return rc;
+  // Vector loads need every row to start on a 16-byte boundary (a lane's 8 values then do, too).
+  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && (row_stride * static_cast<int64_t>(sizeof(T))) % 16 == 0;
+  const T* xt = static_cast<const T*>(x);
+  uint8_t* qb = static_cast<uint8_t*>(q);
+  uint8_t* sb = static_cast<uint8_t*>(scales);
+  if (vec) {
+    quantize_mx4_kernel<T, true><<<grid, kThreads, 0, stream>>>(xt, qb, sb, rows, padded, K, row_stride, chunks);
+  } else {
+    quantize_mx4_kernel<T, false><<<grid, kThreads, 0, stream>>>(xt, qb, sb, rows, padded, K, row_stride, chunks);
+  }
+  b200::count_launch();
+  B200_CUDA_OK(cudaGetLastError());
+  return B200_OK;
+}
+
+template <typename T>
+int launch_dequantize(const void* q, const void* scales, void* out, int64_t rows, int64_t K, cudaStream_t stream) {
+  const int64_t chunks = (K + kChunk - 1) / kChunk;
+  unsigned grid = 0;
+  const int rc = grid_for("dequantize_mx", rows, chunks, &grid);
+  if (rc != B200_OK) return rc;
+  dequantize_mx4_kernel<T><<<grid, kThreads, 0, stream>>>(static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scales), static_cast<T*>(out), rows, K, chunks);
+  b200::count_launch();
+  B200_CUDA_OK(cudaGetLastError());
+  return B200_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int b200_quantize_mx(const void* x, int32_t dtype_x, int64_t rows, int64_t K, int64_t row_stride, int32_t dtype_q, void* q, void* scales_packed, void* stream) {
+  B200_REQUIRE(x != nullptr && q != nullptr && scales_packed != nullptr, "quantize_mx: NULL argument");
+  const int rc = check_shape("quantize_mx", rows, K, dtype_q);
+  if (rc != B200_OK) return rc;
+  B200_REQUIRE(row_stride >= K || rows == 1, "quantize_mx: row_stride=%lld is below K=%lld", (long long)row_stride, (long long)K);
+  B200_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(scales_packed)) & 15u) == 0, "quantize_mx: q and scales must be 16-byte aligned");
+  const uintptr_t eb = dtype_x == B200_F32 ? 4u : 2u;
+  B200_REQUIRE((reinterpret_cast<uintptr_t>(x) & (eb - 1u)) == 0, "quantize_mx: x must be aligned to its elements");
+  const cudaStream_t s = b200::as_stream(stream);
+  switch (dtype_x) {
+    case B200_F32: return launch_quantize<float>(x, q, scales_packed, rows, K, row_stride, s);
+    case B200_BF16: return launch_quantize<__nv_bfloat16>(x, q, scales_packed, rows, K, row_stride, s);
+    case B200_F16: return launch_quantize<__half>(x, q, scales_packed, rows, K, row_stride, s);
+    default: return b200::fail(B200_ERR_INVALID, "quantize_mx: dtype_x=%d is not f32, bf16 or f16", dtype_x);
+  }
+}
+
+int b200_dequantize_mx(const void* q, const void* scales_packed, int32_t dtype_q, int64_t rows, int64_t K, int32_t dtype_out, void* out, void* stream) {
+  B200_REQUIRE(q != nullptr && scales_packed != nullptr && out != nullptr, "dequantize_mx: NULL argument");
+  const int rc = check_shape("dequantize_mx", rows, K, dtype_q);
+  if (rc != B200_OK) return rc;
+  B200_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(scales_packed) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0,
+               "dequantize_mx: q, scales and out must be 16-byte aligned");
+  const cudaStream_t s = b200::as_stream(stream);
+  switch (dtype_out) {
+    case B200_F32: return launch_dequantize<float>(q, scales_packed, out, rows, K, s);
+    case B200_BF16: return launch_dequantize<__nv_bfloat16>(q, scales_packed, out, rows, K, s);
+    case B200_F16: return launch_dequantize<__half>(q, scales_packed, out, rows, K, s);
+    default: return b200::fail(B200_ERR_INVALID, "dequantize_mx: dtype_out=%d is not f32, bf16 or f16", dtype_out);
+  }
+}
+
+}  // extern "C"

@@ -373,6 +373,77 @@ __device__ __forceinline__ void umma_mx_stage(uint32_t tmem_d, uint32_t a_lo, ui
 #undef B200_MX_STAGE_ASM
 #undef B200_MX_MMA
 
+// ---- block-scaled 4-bit floats (kind::mxf4): E2M1 elements, one E8M0 scale per 32 of them ----
+// One MMA consumes 32 bytes = 64 elements of K and therefore two scales per row, which sit in
+// neighbouring bytes of a 32-bit scale column (scale ids 0 and 2).  A 128-byte stage is 256
+// elements = eight scales per row = two scale blocks ("halves") per 128 rows: MMAs 0 and 1 read
+// half 0, MMAs 2 and 3 half 1.  The descriptor has the fields of make_idesc_mx; E2M1 is format 1.
+__host__ __device__ constexpr uint32_t make_idesc_mx4(uint32_t umma_m, uint32_t umma_n) { return make_idesc_mx(1u, 1u, umma_m, umma_n); }
+
+// TMEM columns of one scale set: A 2 halves x 4, B 2 halves x 8 (4 used by a 128-column tile).
+#define B200_MX4_CP(GROUP, SMEM, COL)                                                           \
+  "add.u32 ls, %7, " #SMEM "*32;\n"                                                             \
+  "add.u32 tc, %6, " #COL ";\n"                                                                 \
+  "mov.b64 sd, {ls, %8};\n"                                                                     \
+  "tcgen05.cp.cta_group::" GROUP ".32x128b.warpx4 [tc], sd;\n"
+#define B200_MX4_CP_IF(GROUP, SMEM, COL)                                                        \
+  "add.u32 ls, %7, " #SMEM "*32;\n"                                                             \
+  "add.u32 tc, %6, " #COL ";\n"                                                                 \
+  "mov.b64 sd, {ls, %8};\n"                                                                     \
+  "@q tcgen05.cp.cta_group::" GROUP ".32x128b.warpx4 [tc], sd;\n"
+// MMA J of the stage: skipped when the operands end before its 64 elements of K.
+#define B200_MX4_MMA(GROUP, J, ID, SA, SB)                                                      \
+  "setp.gt.u32 r, %10, " #J ";\n"                                                               \
+  "add.u32 la, %1, " #J "*2;\n"                                                                 \
+  "add.u32 lb, %2, " #J "*2;\n"                                                                 \
+  "add.u32 id, %4, " #ID "*0x40000020;\n"                                                       \
+  "mov.b64 da, {la, %3};\n"                                                                     \
+  "mov.b64 db, {lb, %3};\n"                                                                     \
+  "@r tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%0], da, db, id, [" SA "], [" SB "], q;\n"
+
+#define B200_MX4_STAGE_ASM(GROUP)                                                               \
+  asm volatile(                                                                                 \
+      "{\n"                                                                                     \
+      ".reg .pred p, q, r;\n"                                                                   \
+      ".reg .b64 da, db, sd;\n"                                                                 \
+      ".reg .b32 la, lb, id, ls, tc, ta1, tb0, tb1;\n"                                          \
+      "setp.ne.b32 p, %5, 0;\n"                                                                 \
+      "setp.eq.b32 q, %9, 2;\n"                                                                 \
+      "mov.b64 sd, {%7, %8};\n"                                                                 \
+      "tcgen05.cp.cta_group::" GROUP ".32x128b.warpx4 [%6], sd;\n"                              \
+      B200_MX4_CP(GROUP, 1, 4) B200_MX4_CP(GROUP, 2, 8) B200_MX4_CP(GROUP, 3, 16)               \
+      B200_MX4_CP_IF(GROUP, 4, 12) B200_MX4_CP_IF(GROUP, 5, 20)                                 \
+      "add.u32 ta1, %6, 4;\n"                                                                   \
+      "add.u32 tb0, %6, 8;\n"                                                                   \
+      "add.u32 tb1, %6, 16;\n"                                                                  \
+      "setp.eq.b32 q, 0, 0;\n"                                                                  \
+      "mov.b64 da, {%1, %3};\n"                                                                 \
+      "mov.b64 db, {%2, %3};\n"                                                                 \
+      "tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %4, [%6], [tb0], p;\n" \
+      B200_MX4_MMA(GROUP, 1, 1, "%6", "tb0") B200_MX4_MMA(GROUP, 2, 0, "ta1", "tb1")            \
+      B200_MX4_MMA(GROUP, 3, 1, "ta1", "tb1") "}\n" ::"r"(tmem_d),                               \
+      "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate_first), "r"(sf_tmem), "r"(sf_lo), "r"(sf_hi), "r"(NB), \
+      "r"(mmas)                                                                                 \
+      : "memory")
+
+// One block-scaled 4-bit stage: the scale blocks (A half 0, A half 1, then the two halves of each
+// 128 rows of B, 512 bytes apart) go to TMEM, then the first `mmas` (1..4) MMAs of the stage.
+template <int CTA_GROUP, int NB>
+__device__ __forceinline__ void umma_mx4_stage(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc,
+                                               uint32_t accumulate_first, uint32_t sf_tmem, uint32_t sf_lo, uint32_t mmas) {
+  static_assert(NB == 1 || NB == 2, "one or two 128-row groups of B");
+  constexpr uint32_t sf_hi = smem_desc_hi_scales();
+  if constexpr (CTA_GROUP == 1) {
+    B200_MX4_STAGE_ASM("1");
+  } else {
+    B200_MX4_STAGE_ASM("2");
+  }
+}
+#undef B200_MX4_STAGE_ASM
+#undef B200_MX4_MMA
+#undef B200_MX4_CP_IF
+#undef B200_MX4_CP
+
 // Load 32 consecutive fp32 columns of this thread's TMEM lane (warp w may touch lanes
 // 32*(w%4) .. 32*(w%4)+31; thread i of the warp reads lane base+i).
 __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&v)[32]) {

@@ -119,16 +119,53 @@ def quantize_e4m3(x: np.ndarray) -> tuple[np.ndarray, np.float32]:
     return f32_to_e4m3_bits(x / scale), scale
 
 
+E2M1_MAX = 6.0
+E2M1_TABLE = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0], dtype=np.float32)
+
+
+def f32_to_e2m1_codes(x: np.ndarray) -> np.ndarray:
+    """float32 -> fp4-e2m1 codes 0..15 (uint8, one per element), round-to-nearest-even;
+    magnitudes beyond 6 saturate.  There is no code for NaN: it becomes 0."""
+    x = np.ascontiguousarray(x, dtype=np.float32)
+    a = np.minimum(np.where(np.isnan(x), 0.0, np.abs(x)), E2M1_MAX).astype(np.float64)
+    step = np.where(a < 2.0, 0.5, np.where(a < 4.0, 1.0, 2.0))  # spacing of the grid in the value's binade
+    q = np.rint(a / step) * step
+    code = np.searchsorted(E2M1_TABLE[:8], q.astype(np.float32)).astype(np.uint8)
+    return np.where(np.isnan(x), np.uint8(0), code | (np.signbit(x).astype(np.uint8) << np.uint8(3)))
+
+
+def e2m1_codes_to_f32(codes: np.ndarray) -> np.ndarray:
+    """fp4-e2m1 codes (uint8, one per element) -> float32 (exact)."""
+    return E2M1_TABLE[np.ascontiguousarray(codes, dtype=np.uint8) & 15]
+
+
+def pack_e2m1(codes: np.ndarray) -> np.ndarray:
+    """Two codes per byte along the last axis, the one with the lower index in the low nibble."""
+    codes = np.ascontiguousarray(codes, dtype=np.uint8)
+    return codes[..., 0::2] | (codes[..., 1::2] << np.uint8(4))
+
+
+def unpack_e2m1(packed: np.ndarray) -> np.ndarray:
+    """Inverse of :func:`pack_e2m1`."""
+    packed = np.ascontiguousarray(packed, dtype=np.uint8)
+    return np.stack([packed & 15, packed >> np.uint8(4)], axis=-1).reshape(*packed.shape[:-1], 2 * packed.shape[-1])
+
+
 MX_BLOCK = 32  # elements of K that share one E8M0 scale
-_MX_ELEM = {"e4m3": (8, f32_to_e4m3_bits, e4m3_bits_to_f32), "e5m2": (15, f32_to_e5m2_bits, e5m2_bits_to_f32)}
+MX_NAN_SCALE = 255  # E8M0's NaN
+_MX_ELEM = {"e4m3": (8, f32_to_e4m3_bits, e4m3_bits_to_f32), "e5m2": (15, f32_to_e5m2_bits, e5m2_bits_to_f32),
+            "e2m1": (2, f32_to_e2m1_codes, e2m1_codes_to_f32)}
 
 
 def quantize_mx(x: np.ndarray, elem: str = "e4m3") -> tuple[np.ndarray, np.ndarray]:
     """Block-scaled ("MX") quantisation along the last axis, after the OCP microscaling rule:
     per block of 32 values the shared exponent is ``floor(log2(amax)) - emax`` (emax = 8 for
-    e4m3, 15 for e5m2), clamped to [-127, 127]; elements are ``x / 2**exponent`` rounded to
+    e4m3, 15 for e5m2, 2 for e2m1), clamped to [-127, 127]; elements are ``x / 2**exponent`` rounded to
     nearest even with saturation.  Returns ``(bits [..., K], scales [..., K/32])``, both uint8;
-    a scale byte is the biased exponent (127 = 1.0).  An all-zero block gets scale 127."""
+    a scale byte is the biased exponent (127 = 1.0).  An all-zero block gets scale 127.
+
+    ``elem="e2m1"`` packs two elements per byte (``bits [..., K/2]``, the lower index in the low
+    nibble), and a block that holds a NaN or an infinity gets codes 0 and scale 255 (E8M0's NaN)."""
     emax, enc, _ = _MX_ELEM[elem]
     x = np.ascontiguousarray(x, dtype=np.float32)
     K = x.shape[-1]
@@ -136,17 +173,25 @@ def quantize_mx(x: np.ndarray, elem: str = "e4m3") -> tuple[np.ndarray, np.ndarr
         raise ValueError(f"last axis {K} is not a multiple of {MX_BLOCK}")
     blocks = x.reshape(*x.shape[:-1], K // MX_BLOCK, MX_BLOCK)
     amax = np.abs(blocks).max(axis=-1)
+    bad = ~np.isfinite(amax) & (elem == "e2m1")
+    if bad.any():
+        blocks = np.where(bad[..., None], np.float32(0.0), blocks)
+        amax = np.where(bad, np.float32(0.0), amax)
     _, ex = np.frexp(amax)  # amax = m * 2**ex with m in [0.5, 1): floor(log2(amax)) = ex - 1
     shared = np.clip(np.where(amax > 0, ex - 1 - emax, 0), -127, 127).astype(np.int32)
     scaled = blocks / np.ldexp(np.float32(1.0), shared)[..., None]
-    return enc(scaled.astype(np.float32)).reshape(x.shape), (shared + 127).astype(np.uint8)
+    bits = enc(scaled.astype(np.float32)).reshape(x.shape)
+    scales = np.where(bad, MX_NAN_SCALE, shared + 127).astype(np.uint8)
+    return pack_e2m1(bits) if elem == "e2m1" else bits, scales
 
 
 def dequantize_mx(bits: np.ndarray, scales: np.ndarray, elem: str = "e4m3") -> np.ndarray:
     """float32 values of block-scaled data (exact unless the product leaves the f32 range)."""
     _, _, dec = _MX_ELEM[elem]
-    vals = dec(bits)
-    factor = np.ldexp(np.float32(1.0), np.asarray(scales, dtype=np.int32) - 127)
+    vals = dec(unpack_e2m1(bits) if elem == "e2m1" else bits)
+    scales = np.asarray(scales)
+    nan = (scales == MX_NAN_SCALE) & (elem == "e2m1")
+    factor = np.where(nan, np.float32(np.nan), np.ldexp(np.float32(1.0), np.where(nan, 0, scales.astype(np.int32) - 127)))
     return (vals.reshape(*scales.shape, MX_BLOCK) * factor[..., None]).reshape(vals.shape).astype(np.float32)
 
 
@@ -187,4 +232,10 @@ def from_f32(x: np.ndarray, dtype: str) -> np.ndarray:
 
 
 STORAGE = {"f16": np.float16, "bf16": np.uint16, "e4m3": np.uint8, "e5m2": np.uint8, "i8": np.int8, "i32": np.int32,
-           "f32": np.float32, "mxe4m3": np.uint8, "mxe5m2": np.uint8, "e5m2_e4m3": np.uint8, "e4m3_e5m2": np.uint8}
+           "f32": np.float32, "mxe4m3": np.uint8, "mxe5m2": np.uint8, "e5m2_e4m3": np.uint8, "e4m3_e5m2": np.uint8,
+           "mxe2m1": np.uint8}
+
+
+def stored_k(dtype: str, K: int) -> int:
+    """Storage elements per operand row of ``K`` elements: K, or K/2 bytes for the packed 4-bit type."""
+    return K // 2 if dtype == "mxe2m1" else K

@@ -14,12 +14,12 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import _native as nat
-from .dtypes import STORAGE
+from .dtypes import STORAGE, stored_k
 from .execution import GpuBuffer
 
 DTYPE_CODES = {"f16": nat.F16, "bf16": nat.BF16, "e4m3": nat.E4M3, "f32": nat.F32, "e5m2": nat.E5M2, "i8": nat.I8,
                "i32": nat.I32, "e5m2_e4m3": nat.E5M2_E4M3, "e4m3_e5m2": nat.E4M3_E5M2, "mxe4m3": nat.MXE4M3,
-               "mxe5m2": nat.MXE5M2}
+               "mxe5m2": nat.MXE5M2, "mxe2m1": nat.MXE2M1}
 B_LAYOUT_CODES = {"row_major": nat.B_ROW_MAJOR_NK, "ref_preshuffled": nat.B_REF_PRESHUFFLED, "packed": nat.B_PACKED}
 EPILOGUE_CODES = {"none": nat.EPI_NONE, "bias_relu": nat.EPI_BIAS_RELU, "bias": nat.EPI_BIAS, "relu": nat.EPI_RELU}
 BIAS_AXIS_CODES = {"n": nat.BIAS_AXIS_N, "m": nat.BIAS_AXIS_M}
@@ -249,6 +249,22 @@ def pack_mx_scales(scales_in, scales_packed, rows: int, K: int, stream=None) -> 
     nat.call("b200_pack_mx_scales", _ptr(scales_in), _ptr(scales_packed), int(rows), int(K), _ptr(stream))
 
 
+def quantize_mx(x, dtype_x: str, rows: int, K: int, q, scales_packed, dtype_q: str = "mxe2m1", row_stride: Optional[int] = None,
+                stream=None) -> None:
+    """Device-side quantisation to block-scaled fp4: ``x`` is ``[rows][K]`` of ``dtype_x`` ("f32",
+    "bf16" or "f16"; rows ``row_stride`` elements apart, K by default), ``q`` receives ``[rows][K/2]``
+    bytes and ``scales_packed`` (:func:`mx_scales_bytes`) the scales in the product's streaming
+    order.  Same codes and scales as :func:`aster_b200.dtypes.quantize_mx` with ``elem="e2m1"``."""
+    nat.call("b200_quantize_mx", _ptr(x), DTYPE_CODES[dtype_x], int(rows), int(K), int(K if row_stride is None else row_stride),
+             DTYPE_CODES[dtype_q], _ptr(q), _ptr(scales_packed), _ptr(stream))
+
+
+def dequantize_mx(q, scales_packed, rows: int, K: int, out, dtype_out: str = "f32", dtype_q: str = "mxe2m1", stream=None) -> None:
+    """Device-side inverse of :func:`quantize_mx`: ``[rows][K]`` values of ``dtype_out``."""
+    nat.call("b200_dequantize_mx", _ptr(q), _ptr(scales_packed), DTYPE_CODES[dtype_q], int(rows), int(K), DTYPE_CODES[dtype_out],
+             _ptr(out), _ptr(stream))
+
+
 def _check_operand(name: str, arr: np.ndarray, shape, dtype: str) -> np.ndarray:
     want = STORAGE[dtype]
     if not isinstance(arr, np.ndarray):
@@ -286,19 +302,22 @@ def gemm(
     layout ("ref_preshuffled" or "packed" = row-major to be packed) is packed on the device
     first.  ``tail_split=True`` lends the plan its optional workspace so that a mostly idle
     last round of tiles is cut along K (changes the fp32 summation order of those tiles).
-    For the block-scaled types ("mxe4m3", "mxe5m2") ``block_scales_a`` / ``block_scales_b`` are
-    the E8M0 scale bytes ``[M, K/32]`` / ``[N, K/32]`` (see :func:`aster_b200.dtypes.quantize_mx`).
+    For the block-scaled types ("mxe4m3", "mxe5m2", "mxe2m1") ``block_scales_a`` / ``block_scales_b`` are
+    the E8M0 scale bytes ``[M, K/32]`` / ``[N, K/32]`` (see :func:`aster_b200.dtypes.quantize_mx`);
+    "mxe2m1" operands hold two elements per byte, ``[M, K/2]`` and ``[N, K/2]``.
     Returns ``[M, N]`` float32, bf16 bit patterns (uint16) for ``dtype_c="bf16"``, or the int32
     sums for int8 inputs with ``dtype_c="i32"``.
     """
     if shape is None:
         M, K = A.shape
         N = B.shape[0]
+        if dtype_ab == "mxe2m1":
+            K *= 2
     else:
         M, N, K = shape
     type_a, type_b = dtype_ab.split("_")[0], dtype_ab.split("_")[-1]  # "e5m2_e4m3": A e5m2, B e4m3
-    A = _check_operand("A", A, (M, K), type_a)
-    B = _check_operand("B", B, (N, K), type_b)
+    A = _check_operand("A", A, (M, stored_k(dtype_ab, K)), type_a)
+    B = _check_operand("B", B, (N, stored_k(dtype_ab, K)), type_b)
     if plan is None:
         epilogue = {(False, False): "none", (True, True): "bias_relu", (True, False): "bias", (False, True): "relu"}[
             (bias is not None, bool(relu))
@@ -405,7 +424,7 @@ class HostGemmPipeline:
         res = plan.resources()
         eb_ab = np.dtype(STORAGE[plan.dtype_ab]).itemsize
         eb_c = np.dtype(STORAGE[plan.dtype_c]).itemsize
-        self.a_bytes, self.b_bytes = plan.M * plan.K * eb_ab, plan.N * plan.K * eb_ab
+        self.a_bytes, self.b_bytes = (rows * stored_k(plan.dtype_ab, plan.K) * eb_ab for rows in (plan.M, plan.N))
         self.c_bytes = plan.M * plan.N * eb_c
         nat.init_current()
         self.streams = [GpuStream() for _ in range(depth)]
@@ -429,8 +448,8 @@ class HostGemmPipeline:
 
     def pinned_operands(self):
         """Allocate pinned host arrays for one problem's A and B."""
-        return (PinnedArray((self.plan.M, self.plan.K), STORAGE[self.plan.dtype_ab]),
-                PinnedArray((self.plan.N, self.plan.K), STORAGE[self.plan.dtype_ab]))
+        cols = stored_k(self.plan.dtype_ab, self.plan.K)
+        return (PinnedArray((self.plan.M, cols), STORAGE[self.plan.dtype_ab]), PinnedArray((self.plan.N, cols), STORAGE[self.plan.dtype_ab]))
 
     @property
     def h2d_bytes_per_problem(self) -> int:

@@ -219,7 +219,7 @@ class ShardedHostGemmPipeline:
         import torch
 
         from . import _native as nat
-        from .dtypes import STORAGE
+        from .dtypes import STORAGE, stored_k
         from .execution import GpuBuffer, GpuStream
         from .gemm import PinnedArray
 
@@ -234,8 +234,9 @@ class ShardedHostGemmPipeline:
         eb_c = np.dtype(STORAGE[plan.dtype_c]).itemsize
         self.b_rows = plan.N // world
         self.b_row_slice = slice(rank * self.b_rows, (rank + 1) * self.b_rows)
-        self.a_bytes = plan.M * plan.K * eb_ab
-        self.b_shard_bytes = self.b_rows * plan.K * eb_ab
+        self._cols = stored_k(plan.dtype_ab, plan.K)
+        self.a_bytes = plan.M * self._cols * eb_ab
+        self.b_shard_bytes = self.b_rows * self._cols * eb_ab
         self.c_bytes = plan.M * plan.N * eb_c
         self._b_dtype = STORAGE[plan.dtype_ab]
         nat.init_current()
@@ -268,8 +269,7 @@ class ShardedHostGemmPipeline:
         from .dtypes import STORAGE
         from .gemm import PinnedArray
 
-        return (PinnedArray((self.plan.M, self.plan.K), STORAGE[self.plan.dtype_ab]),
-                PinnedArray((self.b_rows, self.plan.K), self._b_dtype))
+        return (PinnedArray((self.plan.M, self._cols), STORAGE[self.plan.dtype_ab]), PinnedArray((self.b_rows, self._cols), self._b_dtype))
 
     @property
     def h2d_bytes_per_problem(self) -> int:

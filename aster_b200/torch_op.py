@@ -13,10 +13,21 @@ current stream to the C ABI (``b200_gemm_run``), there is no copy and no fallbac
 ``a`` is ``[M, K]``, ``b`` is ``[N, K]`` (both contiguous, K fastest: ``c = a @ b.T``), dtype
 float16, bfloat16 or float8_e4m3fn; ``bias`` is an optional float32 ``[N]``; ``scale_a`` /
 ``scale_b`` are optional one-element float32 CUDA tensors (per-tensor dequantisation scales).
+
+Block-scaled fp4 (OCP MX: E2M1 elements, one power-of-two scale per 32 of them along K):
+
+    q, s = torch.ops.aster_b200.quantize_mx(x)                # [M, K] -> codes [M, K/2], scales
+    c = torch.ops.aster_b200.gemm_mx_nt(q, s, wq, ws, bias, relu=True, out_dtype=torch.bfloat16)
+    x2 = torch.ops.aster_b200.dequantize_mx(q, s, torch.bfloat16)
+
+The codes are uint8, two per byte (the lower K index in the low nibble); the scales are one flat
+uint8 tensor in the order that the product streams them.  Weights are quantised once, activations
+before each product.  Each of the three has a ``..._direct`` twin without the dispatcher's cost.
 """
 
 from __future__ import annotations
 
+import threading
 from typing import Optional
 
 import torch
@@ -121,6 +132,153 @@ def gemm_nt(a: torch.Tensor, b: torch.Tensor, bias: Optional[torch.Tensor] = Non
 
 @gemm_nt.register_fake
 def _(a, b, bias=None, relu=False, out_dtype=torch.float32, scale_a=None, scale_b=None):
+    return a.new_empty((a.shape[0], b.shape[0]), dtype=out_dtype)
+
+
+_MX_VALUE_DTYPES = {torch.float32: nat.F32, torch.bfloat16: nat.BF16, torch.float16: nat.F16}
+# A block-scaled plan is told its scales before each launch: the two steps of a call belong together
+# when several threads share a plan.
+_mx_lock = threading.Lock()
+
+
+def _on_device(device: torch.device, launch) -> None:
+    """Run ``launch`` with ``device`` current (the C ABI works on the current device, like torch)."""
+
+    def ready() -> None:
+        if device.index not in _ready_devices:
+            nat.init_current()
+            _ready_devices.add(device.index)
+        launch()
+
+    if torch.cuda.current_device() == device.index:
+        ready()
+    else:
+        with torch.cuda.device(device):
+            ready()
+
+
+def _mx_scales_bytes(rows: int, K: int) -> int:
+    """What ``b200_mx_scales_bytes`` answers, without the call: 512 bytes per [128 rows][128 of K]."""
+    return (rows + 127) // 128 * ((K + 127) // 128) * 512
+
+
+def _check_mx_operand(name: str, q: torch.Tensor, scales: torch.Tensor) -> None:
+    """Packed codes ``[rows, K/2]`` and their scales, in the layout that ``quantize_mx`` returns."""
+    for what, t in ((name, q), (f"{name}'s scales", scales)):
+        if not t.is_cuda:
+            raise RuntimeError(f"{what} must be a CUDA tensor (there is no CPU path)")
+        if t.dtype != torch.uint8:
+            raise RuntimeError(f"{what} must be uint8, got {t.dtype}")
+    if q.dim() != 2 or q.shape[0] < 1 or q.shape[1] < 16 or q.shape[1] % 16:
+        raise RuntimeError(f"{name} must be packed codes [rows, K/2] with K a positive multiple of 32, got {tuple(q.shape)}")
+    want = _mx_scales_bytes(q.shape[0], 2 * q.shape[1])
+    if scales.device != q.device or scales.dim() != 1 or scales.numel() != want:
+        raise RuntimeError(f"{name}'s scales must be the {want} packed bytes on {q.device} that quantize_mx returns, got {tuple(scales.shape)} on {scales.device}")
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and 16-byte aligned (a view can start anywhere)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def quantize_mx_direct(x: torch.Tensor, elem: str = "e2m1") -> tuple[torch.Tensor, torch.Tensor]:
+    """``x`` ``[M, K]`` (float32, bfloat16 or float16; K a multiple of 32; rows may be strided) to
+    block-scaled fp4: packed codes uint8 ``[M, K/2]`` and the packed scales.  A block of 32 that holds
+    a NaN or an infinity reads as 32 NaN afterwards."""
+    if elem != "e2m1":
+        raise RuntimeError(f"quantize_mx makes e2m1 elements, not {elem!r}")
+    if not x.is_cuda:
+        raise RuntimeError("aster_b200::quantize_mx needs a CUDA tensor (there is no CPU path)")
+    if x.dim() != 2 or x.shape[0] < 1 or x.shape[1] < 32 or x.shape[1] % 32:
+        raise RuntimeError(f"expected x [M, K] with M >= 1 and K a positive multiple of 32, got {tuple(x.shape)}")
+    if x.dtype not in _MX_VALUE_DTYPES:
+        raise RuntimeError(f"unsupported dtype {x.dtype}")
+    M, K = x.shape
+    if x.stride(1) != 1 or (M > 1 and x.stride(0) < K):
+        x = x.contiguous()
+    q = torch.empty((M, K // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(_mx_scales_bytes(M, K), dtype=torch.uint8, device=x.device)
+    _on_device(x.device, lambda: nat.check(nat.lib().b200_quantize_mx(
+        x.data_ptr(), _MX_VALUE_DTYPES[x.dtype], M, K, x.stride(0), nat.MXE2M1, q.data_ptr(), scales.data_ptr(), _raw_stream(x.device))))
+    return q, scales
+
+
+def dequantize_mx_direct(q: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values ``[M, K]`` that packed codes and scales stand for (exact in float32 and bfloat16)."""
+    _check_mx_operand("q", q, scales)
+    if out_dtype not in _MX_VALUE_DTYPES:
+        raise RuntimeError(f"unsupported out_dtype {out_dtype}")
+    q, scales = _aligned(q), _aligned(scales)
+    M, K = q.shape[0], 2 * q.shape[1]
+    out = torch.empty((M, K), dtype=out_dtype, device=q.device)
+    _on_device(q.device, lambda: nat.check(nat.lib().b200_dequantize_mx(
+        q.data_ptr(), scales.data_ptr(), nat.MXE2M1, M, K, _MX_VALUE_DTYPES[out_dtype], out.data_ptr(), _raw_stream(q.device))))
+    return out
+
+
+def gemm_mx_nt_direct(a: torch.Tensor, scales_a: torch.Tensor, b: torch.Tensor, scales_b: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                      relu: bool = False, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """``epilogue(A . B^T)`` of two block-scaled fp4 operands as :func:`quantize_mx_direct` returns
+    them: ``a`` ``[M, K/2]``, ``b`` ``[N, K/2]``, optional float32 ``bias`` ``[N]`` and ReLU, fp32
+    accumulation, ``[M, N]`` out.  The first call of a shape allocates: make it before a stream capture."""
+    _check_mx_operand("a", a, scales_a)
+    _check_mx_operand("b", b, scales_b)
+    if a.device != b.device or a.shape[1] != b.shape[1]:
+        raise RuntimeError(f"expected a [M, K/2] and b [N, K/2] on one device, got {tuple(a.shape)} on {a.device} and {tuple(b.shape)} on {b.device}")
+    if out_dtype not in _OUT_DTYPES:
+        raise RuntimeError(f"unsupported out_dtype {out_dtype}")
+    M, N, K = a.shape[0], b.shape[0], 2 * a.shape[1]
+    if bias is not None and (bias.dtype != torch.float32 or bias.device != a.device or bias.numel() != N):
+        raise RuntimeError(f"bias must be {N} float32 values on {a.device}")
+    a, scales_a, b, scales_b = _aligned(a), _aligned(scales_a), _aligned(b), _aligned(scales_b)
+    bias = None if bias is None else bias.contiguous()
+    device = a.device
+    out = torch.empty((M, N), dtype=out_dtype, device=device)
+
+    def launch() -> None:
+        with _mx_lock:
+            key = (device.index, M, N, K, "mxe2m1", _OUT_DTYPES[out_dtype], _EPILOGUES[(bias is not None, relu)])
+            if key not in _plans:
+                _plans[key] = (GemmPlan(*key[1:6], epilogue=key[6]), None)
+            plan = _plans[key][0]
+            nat.check(nat.lib().b200_gemm_plan_set_mx_scales(plan.handle, scales_a.data_ptr(), scales_b.data_ptr()))
+            nat.check(_gemm_run()(plan.handle, a.data_ptr(), b.data_ptr(), out.data_ptr(), None if bias is None else bias.data_ptr(),
+                                  None, None, None, 0, _raw_stream(device)))
+
+    _on_device(device, launch)
+    return out
+
+
+@torch.library.custom_op("aster_b200::quantize_mx", mutates_args=())
+def quantize_mx(x: torch.Tensor, elem: str = "e2m1") -> tuple[torch.Tensor, torch.Tensor]:
+    return quantize_mx_direct(x, elem)
+
+
+@quantize_mx.register_fake
+def _(x, elem="e2m1"):
+    M, K = x.shape
+    return x.new_empty((M, K // 2), dtype=torch.uint8), x.new_empty((_mx_scales_bytes(M, K),), dtype=torch.uint8)
+
+
+@torch.library.custom_op("aster_b200::dequantize_mx", mutates_args=())
+def dequantize_mx(q: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    return dequantize_mx_direct(q, scales, out_dtype)
+
+
+@dequantize_mx.register_fake
+def _(q, scales, out_dtype=torch.float32):
+    return q.new_empty((q.shape[0], 2 * q.shape[1]), dtype=out_dtype)
+
+
+@torch.library.custom_op("aster_b200::gemm_mx_nt", mutates_args=())
+def gemm_mx_nt(a: torch.Tensor, scales_a: torch.Tensor, b: torch.Tensor, scales_b: torch.Tensor, bias: Optional[torch.Tensor] = None,
+               relu: bool = False, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    return gemm_mx_nt_direct(a, scales_a, b, scales_b, bias, relu, out_dtype)
+
+
+@gemm_mx_nt.register_fake
+def _(a, scales_a, b, scales_b, bias=None, relu=False, out_dtype=torch.float32):
     return a.new_empty((a.shape[0], b.shape[0]), dtype=out_dtype)
 
 

@@ -114,7 +114,11 @@ enum {
    * (include/aster/Dialect/AMDGCN/IR/Instructions/MMA.td; test/integration/
    * test_mfma_f8f6f4_e2e.py:39-95).  Scales are attached with b200_gemm_plan_set_mx_scales. */
   B200_MXE4M3 = 9,
-  B200_MXE5M2 = 10
+  B200_MXE5M2 = 10,
+  /* Block-scaled fp4 (OCP MX: E2M1 elements, magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6, with the same
+   * scales): two elements per byte, the one with the lower K index in the low nibble, so a row
+   * of A or B is K/2 bytes.  b200_quantize_mx makes such operands on the device. */
+  B200_MXE2M1 = 11
 };
 /* Layout of the B operand handed to b200_pack_b / b200_gemm_run. */
 enum {
@@ -127,7 +131,8 @@ enum { B200_BIAS_AXIS_N = 0, B200_BIAS_AXIS_M = 1 };
 
 typedef struct b200_gemm_desc {
   int64_t M, N, K;
-  int32_t dtype_ab;  /* B200_F16 | B200_BF16 | B200_E4M3 | B200_E5M2 | the two mixes | B200_I8   */
+  int32_t dtype_ab;  /* B200_F16 | B200_BF16 | B200_E4M3 | B200_E5M2 | the two mixes | B200_I8
+                      * | the block-scaled types                                                */
   int32_t dtype_c;   /* B200_F32 | B200_BF16 | B200_I32 (i8 inputs, no epilogue, no scales)     */
   int32_t b_layout;  /* B200_B_*                                                                */
   int32_t epilogue;  /* B200_EPI_*                                                              */
@@ -279,7 +284,7 @@ int b200_copy_2d_padded_f32(const float* src, float* dst, int64_t M, int64_t N, 
 /* out[i] = max(a[i] + b[i], 0); examples/07_simple_fusion/simple_fusion.py:62-144. */
 int b200_add_relu_f32(const float* a, const float* b, float* out, size_t n, void* stream);
 
-/* ---- block-scaled fp8 (dtype_ab = B200_MXE4M3 | B200_MXE5M2) -----------------------------
+/* ---- block-scaled fp8 and fp4 (dtype_ab = B200_MXE4M3 | B200_MXE5M2 | B200_MXE2M1) --------
  * C = (A * 2^(sa-127)) . (B * 2^(sb-127))^T with sa[M][K/32], sb[N][K/32] bytes.  K % 32 == 0;
  * row-major B; tile_n 128 or 256.  The kernel streams the scales in blocks of
  * [128 rows][4 K blocks]; b200_pack_mx_scales turns row-major scales (device memory,
@@ -290,6 +295,19 @@ int b200_add_relu_f32(const float* a, const float* b, float* out, size_t n, void
 int b200_mx_scales_bytes(int64_t rows, int64_t K, size_t* bytes);
 int b200_pack_mx_scales(const void* scales_in, void* scales_packed, int64_t rows, int64_t K, void* stream);
 int b200_gemm_plan_set_mx_scales(b200_gemm_plan* plan, const void* scales_a_packed, const void* scales_b_packed);
+
+/* Values to block-scaled fp4 on the device and back (no counterpart in the reference).
+ * x: [rows][K] of dtype_x (B200_F32 | B200_BF16 | B200_F16), rows `row_stride` elements apart;
+ * q: [rows][K/2] bytes; scales_packed: b200_mx_scales_bytes(rows, K) bytes in the order that the
+ * product streams (rows behind the last and blocks behind K get byte 127).  Per block of 32 the
+ * shared exponent is floor(log2 max|x|) - 2, clamped to [-127, 127] (a block of zeros: 0), the
+ * elements are x / 2^exponent rounded to nearest even and saturated at 6.  A block that holds a NaN
+ * or an infinity gets scale byte 255: its 32 values read as NaN.  dtype_q = B200_MXE2M1.
+ * q, scales_packed and out are 16-byte aligned; out is [rows][K] of dtype_out. */
+int b200_quantize_mx(const void* x, int32_t dtype_x, int64_t rows, int64_t K, int64_t row_stride, int32_t dtype_q,
+                     void* q, void* scales_packed, void* stream);
+int b200_dequantize_mx(const void* q, const void* scales_packed, int32_t dtype_q, int64_t rows, int64_t K, int32_t dtype_out,
+                       void* out, void* stream);
 
 /* ---- optional: gather row shards of C onto every GPU (NCCL over NVLink) ------------------
  * No counterpart in the reference, whose multi-GPU support is fan-out of whole configurations
