@@ -33,6 +33,8 @@ F16, BF16, E4M3, F32, E5M2, I8, I32, E5M2_E4M3, E4M3_E5M2, MXE4M3, MXE5M2, MXE2M
 B_ROW_MAJOR_NK, B_REF_PRESHUFFLED, B_PACKED = 0, 1, 2
 EPI_NONE, EPI_BIAS_RELU, EPI_BIAS, EPI_RELU = 0, 1, 2, 3
 BIAS_AXIS_N, BIAS_AXIS_M = 0, 1
+HEAD_CROSS_ENTROPY, HEAD_DISTILL = 0, 1
+REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
 
 
 class B200Error(RuntimeError):
@@ -109,6 +111,39 @@ class GemmResources(C.Structure):
     ]
 
 
+class HeadDesc(C.Structure):
+    _fields_ = [
+        ("tokens", C.c_int64),
+        ("hidden", C.c_int64),
+        ("vocab", C.c_int64),
+        ("x_stride", C.c_int64),
+        ("w_stride", C.c_int64),
+        ("ignore_index", C.c_int64),
+        ("kind", C.c_int32),
+        ("dtype", C.c_int32),
+        ("reduction", C.c_int32),
+        ("index_bits", C.c_int32),
+        ("top", C.c_int32),
+        ("dtype_teacher", C.c_int32),
+        ("label_smoothing", C.c_float),
+        ("temperature", C.c_float),
+        ("grad_bytes", C.c_int64),
+    ]
+
+
+class HeadSizes(C.Structure):
+    _fields_ = [
+        ("forward_workspace", C.c_size_t),
+        ("backward_workspace", C.c_size_t),
+        ("saved", C.c_size_t),
+        ("grad_columns", C.c_int64),
+        ("grad_splits", C.c_int32),
+        ("cta_group", C.c_int32),
+        ("tile_n", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
 _P = C.c_void_p
 _SZ = C.c_size_t
 _FP = C.POINTER(C.c_float)
@@ -165,6 +200,10 @@ SIGNATURES = {
     "b200_gemm_plan_set_mx_scales": [_P, _P, _P],
     "b200_quantize_mx": [_P, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_int32, _P, _P, _P],
     "b200_dequantize_mx": [_P, _P, C.c_int32, C.c_int64, C.c_int64, C.c_int32, _P, _P],
+    "b200_head_loss_sizes": [C.POINTER(HeadDesc), C.POINTER(HeadSizes)],
+    "b200_head_loss_forward": [C.POINTER(HeadDesc), _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+    "b200_head_loss_backward": [C.POINTER(HeadDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+    "b200_head_loss_status": [C.POINTER(C.c_uint32)],
     "b200_nccl_version": [C.POINTER(C.c_int)],
     "b200_nccl_init_all": [C.c_int, C.POINTER(C.c_int), C.POINTER(_P)],
     "b200_nccl_destroy": [_P],

@@ -19,8 +19,8 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libaster_b200.so"
 BRINGUP_LIB_PATH = PKG_DIR / "libaster_b200_bringup.so"
-SOURCES = ["runtime.cpp", "nccl_rows.cpp", "bandwidth.cu", "gemm_sm100.cu", "gemm_noalloc.cu", "mx_quant.cu"]
-HEADERS = ["common.h", "ptx_sm100.cuh", "gemm_kernel.cuh", "../../include/aster_b200.h", "../../include/aster_b200_bringup.h"]
+SOURCES = ["runtime.cpp", "nccl_rows.cpp", "bandwidth.cu", "gemm_sm100.cu", "gemm_noalloc.cu", "mx_quant.cu", "head_loss.cu"]
+HEADERS = ["common.h", "ptx_sm100.cuh", "gemm_kernel.cuh", "head_kernel.cuh", "../../include/aster_b200.h", "../../include/aster_b200_bringup.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

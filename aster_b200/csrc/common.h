@@ -29,6 +29,8 @@ inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s
 // box_rows x 128 bytes with the 128-byte swizzle; out-of-range parts of a box read as zero.
 // Defined in gemm_sm100.cu.
 int make_operand_map(CUtensorMap* map, const void* base, int dtype, uint64_t rows, uint64_t cols, uint32_t box_rows);
+// Same with rows `row_stride` elements apart (a multiple of 16 bytes).
+int make_strided_operand_map(CUtensorMap* map, const void* base, int dtype, uint64_t rows, uint64_t cols, uint64_t row_stride, uint32_t box_rows);
 
 }  // namespace b200
 

@@ -48,6 +48,10 @@ EncodeTiledFn encode_tiled_fn() {
 // box_rows x (128 bytes of columns), written to shared memory with the 128-byte swizzle.
 // Out-of-range parts of a box read as zero, which is what makes ragged M, N and K safe.
 int b200::make_operand_map(CUtensorMap* map, const void* base, int dtype, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+  return make_strided_operand_map(map, base, dtype, rows, cols, cols, box_rows);
+}
+
+int b200::make_strided_operand_map(CUtensorMap* map, const void* base, int dtype, uint64_t rows, uint64_t cols, uint64_t row_stride, uint32_t box_rows) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (fn == nullptr) return b200::fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   CUtensorMapDataType dt;
@@ -58,7 +62,7 @@ int b200::make_operand_map(CUtensorMap* map, const void* base, int dtype, uint64
     default: dt = CU_TENSOR_MAP_DATA_TYPE_UINT8; eb = 1; break;
   }
   cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {cols * eb};
+  cuuint64_t strides[1] = {row_stride * eb};
   cuuint32_t box[2] = {static_cast<cuuint32_t>(gemm::kRowBytes / eb), box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,

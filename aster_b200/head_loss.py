@@ -1,0 +1,315 @@
+"""Losses of a language model's head on torch tensors, without the logits.
+
+The head's product ``z = x . w^T`` (``x`` ``[tokens, hidden]``, ``w`` ``[vocab, hidden]``, the ``gemm_nt``
+layout) is consumed tile by tile where the tensor cores leave it: the forward pass keeps a maximum and
+a sum per row, the backward pass computes z again, a range of the vocabulary at a time, and turns it into
+both gradients.  Nothing of size ``tokens x vocab`` is ever stored but that range of ``dL/dz`` in 16 bits.
+
+    from aster_b200.head_loss import linear_cross_entropy, linear_distillation
+
+    loss = linear_cross_entropy(x, w, target, label_smoothing=0.1)     # differentiable in x and w
+    loss = linear_distillation(x, w, teacher_logits, teacher_ids, temperature=2.0)
+
+``torch.ops.aster_b200.linear_cross_entropy`` / ``linear_distillation`` are the same as operators of the
+dispatcher (they return ``(loss, lse, saved)``; ``loss`` is differentiable).  The tensors only lend their
+storage to ``b200_head_loss_*``; torch's current stream is used, there is no CPU path and no fallback.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Sequence
+
+import torch
+
+from . import _native as nat
+from .torch_op import _on_device, _raw_stream
+
+_DTYPES = {torch.bfloat16: nat.BF16, torch.float16: nat.F16}
+_TEACHER_DTYPES = {torch.float32: nat.F32, torch.bfloat16: nat.BF16, torch.float16: nat.F16}
+_INDEX_BITS = {torch.int64: 64, torch.int32: 32}
+_REDUCTIONS = {"none": nat.REDUCE_NONE, "mean": nat.REDUCE_MEAN, "sum": nat.REDUCE_SUM}
+MAX_TOP = 1024  # teacher entries per row
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """Two dimensions, the last one contiguous, rows a multiple of 16 bytes apart and aligned (else a copy)."""
+    t = t.reshape(-1, t.shape[-1])
+    if t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1])):
+        t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _check(name: str, x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, reduction: str) -> None:
+    for what, t in (("x", x), ("weight", w), ("labels", labels)):
+        if not t.is_cuda:
+            raise RuntimeError(f"aster_b200::{name} needs CUDA tensors, {what} is on {t.device} (there is no CPU path)")
+        if t.device != x.device:
+            raise RuntimeError(f"{what} is on {t.device}, x on {x.device}")
+    if x.dtype not in _DTYPES or w.dtype != x.dtype:
+        raise RuntimeError(f"unsupported dtypes {x.dtype}, {w.dtype}: both bfloat16 or both float16")
+    if x.dim() < 2 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
+        raise RuntimeError(f"expected x [..., hidden] and weight [vocab, hidden], got {tuple(x.shape)} and {tuple(w.shape)}")
+    if w.shape[0] < 1 or w.shape[1] < 8 or w.shape[1] % 8:
+        raise RuntimeError(f"weight {tuple(w.shape)}: vocab must be at least 1 and hidden a positive multiple of 8")
+    if labels.dtype not in _INDEX_BITS:
+        raise RuntimeError(f"labels must be int64 or int32, got {labels.dtype}")
+    if reduction not in _REDUCTIONS:
+        raise RuntimeError(f"unknown reduction {reduction!r}")
+
+
+def _desc(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, reduction: str) -> nat.HeadDesc:
+    d = nat.HeadDesc()
+    d.tokens, d.hidden = x.shape
+    d.vocab = w.shape[0]
+    d.x_stride = x.stride(0) if d.tokens > 1 else d.hidden
+    d.w_stride = w.stride(0) if d.vocab > 1 else d.hidden
+    d.dtype, d.reduction, d.index_bits = _DTYPES[x.dtype], _REDUCTIONS[reduction], _INDEX_BITS[labels.dtype]
+    return d
+
+
+def _sizes(d: nat.HeadDesc) -> nat.HeadSizes:
+    s = nat.HeadSizes()
+    nat.call("b200_head_loss_sizes", C.byref(d), C.byref(s))
+    return s
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+class _Head:
+    """One call's tensors as the C ABI wants them, and its description."""
+
+    def __init__(self, x, w, labels, reduction, *, kind, ignore_index=0, label_smoothing=0.0, temperature=1.0, teacher=None, grad_bytes=0):
+        self.x, self.w, self.labels, self.teacher = _rows(x), _rows(w), labels.contiguous(), teacher
+        self.desc = d = _desc(self.x, self.w, labels, reduction)
+        d.kind, d.ignore_index, d.label_smoothing, d.temperature = kind, ignore_index, label_smoothing, temperature
+        d.grad_bytes = grad_bytes
+        if kind == nat.HEAD_DISTILL:
+            d.top, d.dtype_teacher = labels.shape[-1], nat.F32 if teacher is None else _TEACHER_DTYPES[teacher.dtype]
+        self.per_row = reduction == "none"
+
+    def forward(self):
+        dev, tokens = self.x.device, self.x.shape[0]
+        f32 = dict(dtype=torch.float32, device=dev)
+        if tokens == 0:  # nothing to launch
+            loss = torch.empty(0, **f32) if self.per_row else torch.full((), float("nan") if self.desc.reduction == nat.REDUCE_MEAN else 0.0, **f32)
+            return loss, torch.empty(0, **f32), torch.empty(0, dtype=torch.uint8, device=dev)
+        sizes = _sizes(self.desc)
+        loss = torch.empty(tokens if self.per_row else (), **f32)
+        lse = torch.empty(tokens, **f32)
+        saved = torch.empty(sizes.saved, dtype=torch.uint8, device=dev)
+        ws = torch.empty(sizes.forward_workspace, dtype=torch.uint8, device=dev)
+        _on_device(dev, lambda: nat.call("b200_head_loss_forward", C.byref(self.desc), self.x.data_ptr(), self.w.data_ptr(), self.labels.data_ptr(),
+                                         _ptr(self.teacher), loss.data_ptr(), lse.data_ptr(), saved.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(dev)))
+        return loss, lse, saved
+
+    def backward(self, grad, lse, saved, want_x: bool, want_w: bool):
+        dev, tokens = self.x.device, self.x.shape[0]
+        dx = torch.empty(self.x.shape, dtype=self.x.dtype, device=dev) if want_x else None
+        if tokens == 0:
+            return dx, torch.zeros(self.w.shape, dtype=self.w.dtype, device=dev) if want_w else None
+        dw = torch.empty(self.w.shape, dtype=self.w.dtype, device=dev) if want_w else None
+        grad = grad.to(torch.float32).contiguous()
+        ws = torch.empty(_sizes(self.desc).backward_workspace, dtype=torch.uint8, device=dev)
+        _on_device(dev, lambda: nat.call("b200_head_loss_backward", C.byref(self.desc), self.x.data_ptr(), self.w.data_ptr(), self.labels.data_ptr(),
+                                         lse.data_ptr(), saved.data_ptr(), grad.data_ptr(), _ptr(dx), _ptr(dw), ws.data_ptr(), ws.numel(), _raw_stream(dev)))
+        return dx, dw
+
+
+def _xent_head(x, w, target, ignore_index, label_smoothing, reduction, grad_bytes=0) -> _Head:
+    _check("linear_cross_entropy", x, w, target, reduction)
+    if target.shape != x.shape[:-1]:
+        raise RuntimeError(f"target {tuple(target.shape)} does not match x {tuple(x.shape)}")
+    if not 0.0 <= label_smoothing < 1.0:
+        raise RuntimeError(f"label_smoothing={label_smoothing} is outside [0, 1)")
+    return _Head(x, w, target, reduction, kind=nat.HEAD_CROSS_ENTROPY, ignore_index=ignore_index, label_smoothing=label_smoothing, grad_bytes=grad_bytes)
+
+
+def _distill_head(x, w, teacher_logits, teacher_ids, temperature, reduction, grad_bytes=0) -> _Head:
+    _check("linear_distillation", x, w, teacher_ids, reduction)
+    if teacher_ids.dim() != x.dim() or teacher_ids.shape[:-1] != x.shape[:-1] or not 1 <= teacher_ids.shape[-1] <= MAX_TOP:
+        raise RuntimeError(f"teacher_ids {tuple(teacher_ids.shape)} do not match x {tuple(x.shape)} with 1 to {MAX_TOP} entries per row")
+    if teacher_logits is not None:
+        if teacher_logits.shape != teacher_ids.shape or teacher_logits.device != x.device:
+            raise RuntimeError(f"teacher_logits {tuple(teacher_logits.shape)} on {teacher_logits.device} do not match teacher_ids {tuple(teacher_ids.shape)} on {x.device}")
+        if teacher_logits.dtype not in _TEACHER_DTYPES:
+            raise RuntimeError(f"unsupported teacher_logits dtype {teacher_logits.dtype}")
+        teacher_logits = teacher_logits.detach().contiguous()
+    if not 0.0 < temperature < float("inf"):
+        raise RuntimeError(f"temperature={temperature} must be positive and finite")
+    return _Head(x, w, teacher_ids, reduction, kind=nat.HEAD_DISTILL, temperature=temperature, teacher=teacher_logits, grad_bytes=grad_bytes)
+
+
+_STREAM_NOTE = "aster_b200.stream"
+
+
+def _note_leaves(*tensors: torch.Tensor) -> list:
+    """Autograd keeps one accumulation node per leaf, tied to the stream that was current when it was made,
+    for as long as any graph refers to it.  A backward pass that is being captured cannot join the default
+    stream, so a graph left over from there would break the capture (and, from the engine's own threads, the
+    process).  The node remembers its stream here, and such a capture is refused before it begins.  The
+    caller holds the returned nodes until its own graph refers to them."""
+    nodes = []
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad and t.is_leaf:
+                node = torch.autograd.graph.get_gradient_edge(t).node
+                stream = torch.cuda.current_stream(t.device).cuda_stream
+                if node.metadata.setdefault(_STREAM_NOTE, stream) == 0 and stream != 0 and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("an autograd graph of the same leaf, made on the default stream, is still alive: its backward pass cannot be "
+                                       "captured; free that graph (delete its loss) before the capture")
+                nodes.append(node)
+    return nodes
+
+
+class _HeadLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, head, shape):
+        loss, lse, saved = head.forward()
+        # the tensors come back through save_for_backward: it notices a change in place before the backward pass
+        ctx.save_for_backward(x, w, head.labels, lse, saved)
+        ctx.desc_args, ctx.shape = head.desc, x.shape
+        ctx.per_row = head.per_row
+        return loss.view(shape) if head.per_row else loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, w, labels, lse, saved = ctx.saved_tensors
+        head = _Head.__new__(_Head)
+        head.x, head.w, head.labels, head.teacher, head.desc, head.per_row = _rows(x), _rows(w), labels, None, ctx.desc_args, ctx.per_row
+        dx, dw = head.backward(grad, lse, saved, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return None if dx is None else dx.view(ctx.shape), dw, None, None
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100, label_smoothing: float = 0.0,
+                         reduction: str = "mean", grad_bytes: int = 0) -> torch.Tensor:
+    """Softmax cross entropy of ``x . weight^T`` against ``target``, as
+    ``torch.nn.functional.cross_entropy`` defines it, in fp32, differentiable in ``x`` and ``weight``.
+
+    ``x`` ``[..., hidden]`` and ``weight`` ``[vocab, hidden]`` are both bfloat16 or both float16 (hidden a
+    multiple of 8), ``target`` ``[...]`` int64 or int32.  Targets equal to ``ignore_index`` have no loss and
+    no gradient; any other target outside the vocabulary makes its loss, and the gradients it enters, NaN.
+    "mean" divides by the number of targets that count (NaN without any).  ``grad_bytes`` limits what the
+    backward pass keeps of ``dL/dz`` at a time (0: 256 MiB)."""
+    head = _xent_head(x, weight, target, ignore_index, label_smoothing, reduction, grad_bytes)
+    leaves = _note_leaves(x, weight)
+    loss = _HeadLoss.apply(x, weight, head, target.shape)
+    del leaves
+    return loss
+
+
+def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor, *, temperature: float = 1.0,
+                        reduction: str = "mean", grad_bytes: int = 0) -> torch.Tensor:
+    """Distillation of the head ``x . weight^T`` from a teacher's top logits: per row
+    ``T^2 * KL(softmax(teacher_logits / T) || softmax(x . weight^T / T))`` with the teacher's distribution over
+    its ``teacher_ids`` alone, in fp32, differentiable in ``x`` and ``weight`` (not in the teacher).
+
+    ``teacher_logits`` (float32, bfloat16 or float16) and ``teacher_ids`` (int64 or int32) are ``[..., top]``, in any
+    order, ``top`` at most 1024.  Entries with a negative id or a logit of minus infinity are left out; rows with
+    nothing left have no loss and no gradient and do not count for "mean".  An id listed twice counts twice; an
+    id beyond the vocabulary, or a logit that is NaN or plus infinity, makes the row NaN."""
+    head = _distill_head(x, weight, teacher_logits, teacher_ids, temperature, reduction, grad_bytes)
+    leaves = _note_leaves(x, weight)
+    loss = _HeadLoss.apply(x, weight, head, teacher_ids.shape[:-1])
+    del leaves
+    return loss
+
+
+def head_loss_status() -> Sequence[int]:
+    """Status words of the calls made so far on the current device (synchronises it); raises
+    ``B200Error`` (TIMEOUT) if a bounded device-side wait gave up."""
+    words = (C.c_uint32 * 4)()
+    nat.call("b200_head_loss_status", words)
+    return list(words)
+
+
+# ---- operators of the dispatcher ----
+def _fake_outputs(x, reduction, rows_shape, saved):
+    loss = x.new_empty(rows_shape if reduction == "none" else (), dtype=torch.float32)
+    return loss, x.new_empty((x.numel() // x.shape[-1],), dtype=torch.float32), x.new_empty((saved,), dtype=torch.uint8)
+
+
+def _align256(n: int) -> int:
+    return (n + 255) // 256 * 256
+
+
+@torch.library.custom_op("aster_b200::linear_cross_entropy", mutates_args=())
+def _xent_op(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100, label_smoothing: float = 0.0,
+             reduction: str = "mean") -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    head = _xent_head(x, weight, target, ignore_index, label_smoothing, reduction)
+    loss, lse, saved = head.forward()
+    return loss.view(target.shape) if head.per_row else loss, lse, saved
+
+
+@_xent_op.register_fake
+def _(x, weight, target, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
+    return _fake_outputs(x, reduction, target.shape, 256 if x.numel() else 0)
+
+
+@torch.library.custom_op("aster_b200::linear_cross_entropy_backward", mutates_args=())
+def _xent_backward_op(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, saved: torch.Tensor,
+                      ignore_index: int, label_smoothing: float, reduction: str) -> tuple[torch.Tensor, torch.Tensor]:
+    dx, dw = _xent_head(x, weight, target, ignore_index, label_smoothing, reduction).backward(grad, lse, saved, True, True)
+    return dx.view(x.shape), dw
+
+
+@_xent_backward_op.register_fake
+def _(grad, x, weight, target, lse, saved, ignore_index, label_smoothing, reduction):
+    return x.new_empty(x.shape), weight.new_empty(weight.shape)
+
+
+def _xent_setup(ctx, inputs, output):
+    x, weight, target, ctx.ignore_index, ctx.label_smoothing, ctx.reduction = inputs
+    ctx.mark_non_differentiable(output[1], output[2])
+    ctx.save_for_backward(x, weight, target, output[1], output[2])
+
+
+def _xent_autograd(ctx, grad, _lse, _saved):
+    dx, dw = torch.ops.aster_b200.linear_cross_entropy_backward(grad, *ctx.saved_tensors, ctx.ignore_index, ctx.label_smoothing, ctx.reduction)
+    return dx, dw, None, None, None, None
+
+
+_xent_op.register_autograd(_xent_autograd, setup_context=_xent_setup)
+
+
+@torch.library.custom_op("aster_b200::linear_distillation", mutates_args=())
+def _distill_op(x: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor, temperature: float = 1.0,
+                reduction: str = "mean") -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    head = _distill_head(x, weight, teacher_logits, teacher_ids, temperature, reduction)
+    loss, lse, saved = head.forward()
+    return loss.view(teacher_ids.shape[:-1]) if head.per_row else loss, lse, saved
+
+
+@_distill_op.register_fake
+def _(x, weight, teacher_logits, teacher_ids, temperature=1.0, reduction="mean"):
+    rows, top = x.numel() // x.shape[-1], teacher_ids.shape[-1]
+    return _fake_outputs(x, reduction, teacher_ids.shape[:-1], 256 + _align256(4 * rows) + 2 * _align256(4 * rows * top) if rows else 0)
+
+
+@torch.library.custom_op("aster_b200::linear_distillation_backward", mutates_args=())
+def _distill_backward_op(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, lse: torch.Tensor, saved: torch.Tensor,
+                         temperature: float, reduction: str) -> tuple[torch.Tensor, torch.Tensor]:
+    dx, dw = _distill_head(x, weight, None, teacher_ids, temperature, reduction).backward(grad, lse, saved, True, True)
+    return dx.view(x.shape), dw
+
+
+@_distill_backward_op.register_fake
+def _(grad, x, weight, teacher_ids, lse, saved, temperature, reduction):
+    return x.new_empty(x.shape), weight.new_empty(weight.shape)
+
+
+def _distill_setup(ctx, inputs, output):
+    x, weight, _, teacher_ids, ctx.temperature, ctx.reduction = inputs
+    ctx.mark_non_differentiable(output[1], output[2])
+    ctx.save_for_backward(x, weight, teacher_ids, output[1], output[2])
+
+
+def _distill_autograd(ctx, grad, _lse, _saved):
+    dx, dw = torch.ops.aster_b200.linear_distillation_backward(grad, *ctx.saved_tensors, ctx.temperature, ctx.reduction)
+    return dx, dw, None, None, None, None
+
+
+_distill_op.register_autograd(_distill_autograd, setup_context=_distill_setup)

@@ -309,6 +309,70 @@ int b200_quantize_mx(const void* x, int32_t dtype_x, int64_t rows, int64_t K, in
 int b200_dequantize_mx(const void* q, const void* scales_packed, int32_t dtype_q, int64_t rows, int64_t K, int32_t dtype_out,
                        void* out, void* stream);
 
+/* ---- the loss of a language model's head ---------------------------------------------------
+ * z = x . w^T with x [tokens, hidden] and w [vocab, hidden] (16-bit, K contiguous) feeds a softmax
+ * over the vocabulary; the losses and both gradients come without ever storing z.  (No counterpart in
+ * the reference: the product is its GEMM, the ending takes the place of the fused epilogue of
+ * examples/07_simple_fusion.)
+ *
+ *  cross entropy   L_t = lse(z_t) - (1 - s) z_t[y_t] - s / vocab * sum_v z_t[v]      s = label_smoothing
+ *      target: [tokens] int64 or int32.  A target equal to ignore_index has no loss and no gradient; any
+ *      other target outside [0, vocab) makes its loss and the gradients it enters NaN.
+ *  distillation    L_t = T^2 * sum_j p_tj (log p_tj - log softmax(z_t / T)[id_tj])     T = temperature
+ *      teacher_ids: [tokens][top] int64 or int32, teacher_logits: [tokens][top] f32, bf16 or f16;
+ *      p_t = softmax(teacher_logits_t / T) over the listed entries.  Entries with a negative id or a logit
+ *      of minus infinity are left out; a row with nothing left has no loss and no gradient.  An id listed
+ *      twice counts twice.  An id >= vocab, or a NaN or plus infinity, makes the row's loss and gradients NaN.
+ *
+ * reduction: NONE gives loss [tokens], MEAN divides the sum by the number of rows that have a loss (NaN
+ * when there is none), SUM does not; the latter two give one fp32.  lse [tokens] (natural logarithm of
+ * the sum of exp(z / T)) and `saved` are what the backward pass needs again, beside the same inputs.
+ * grad_loss: [tokens] fp32 for NONE, else one fp32.  grad_x [tokens][hidden] and grad_w [vocab][hidden] are
+ * 16-bit like the operands, contiguous; either may be NULL (not wanted).  Sums over hidden, tokens and the
+ * vocabulary are fp32; the gradient of z is rounded to 16 bits once before the last two products (fp16:
+ * under a common power of two, so that small probabilities keep their digits).  Every result is the same
+ * from run to run.
+ * hidden: a multiple of 8, below 2^31; x, w, grad_x, grad_w, saved and the workspaces 16-byte aligned, rows of x and w
+ * a multiple of 8 elements apart.  Workspaces and `saved` may hold anything before a call.  All calls are
+ * ordered on `stream` and may be recorded into a CUDA graph (make the first call on a device before a
+ * capture: it looks up the status words); nothing is allocated or kept. */
+enum { B200_HEAD_CROSS_ENTROPY = 0, B200_HEAD_DISTILL = 1 };
+enum { B200_REDUCE_NONE = 0, B200_REDUCE_MEAN = 1, B200_REDUCE_SUM = 2 };
+
+typedef struct b200_head_desc {
+  int64_t tokens, hidden, vocab;
+  int64_t x_stride, w_stride;  /* elements between rows                                         */
+  int64_t ignore_index;        /* cross entropy                                                 */
+  int32_t kind;                /* B200_HEAD_*                                                   */
+  int32_t dtype;               /* of x, w and the gradients: B200_F16 | B200_BF16               */
+  int32_t reduction;           /* B200_REDUCE_*                                                 */
+  int32_t index_bits;          /* 64 or 32: target / teacher_ids                                */
+  int32_t top;                 /* distillation: entries per row, 1..1024                        */
+  int32_t dtype_teacher;       /* distillation: B200_F32 | B200_BF16 | B200_F16                 */
+  float label_smoothing;       /* cross entropy: [0, 1)                                         */
+  float temperature;           /* distillation: > 0                                             */
+  int64_t grad_bytes;          /* limit of the stored range of dL/dz; 0 = 256 MiB               */
+} b200_head_desc;
+
+typedef struct b200_head_sizes {
+  size_t forward_workspace, backward_workspace, saved;
+  int64_t grad_columns; /* columns of the vocabulary whose dL/dz is stored at a time            */
+  int32_t grad_splits;  /* parts that the vocabulary axis of grad_x is cut into per range       */
+  int32_t cta_group;    /* 1 or 2 CTAs per MMA                                                  */
+  int32_t tile_n;       /* columns per tile of the forward pass                                 */
+  int32_t reserved;
+} b200_head_sizes;
+
+int b200_head_loss_sizes(const b200_head_desc* desc, b200_head_sizes* sizes);
+/* labels: target or teacher_ids; teacher_logits: NULL for cross entropy. */
+int b200_head_loss_forward(const b200_head_desc* desc, const void* x, const void* w, const void* labels, const void* teacher_logits,
+                           float* loss, float* lse, void* saved, void* workspace, size_t workspace_bytes, void* stream);
+int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const void* w, const void* labels, const float* lse, const void* saved,
+                            const float* grad_loss, void* grad_x, void* grad_w, void* workspace, size_t workspace_bytes, void* stream);
+/* Did every bounded device-side wait of the calls made so far on the current device complete?
+ * (Synchronises it.)  words[0] = 0, else a code naming the wait and B200_ERR_TIMEOUT. */
+int b200_head_loss_status(uint32_t words[4]);
+
 /* ---- optional: gather row shards of C onto every GPU (NCCL over NVLink) ------------------
  * No counterpart in the reference, whose multi-GPU support is fan-out of whole configurations
  * over worker processes (contrib/kittens/test/bench/bench_harness.py:1013-1053).  One process
