@@ -95,7 +95,7 @@ struct Params {
   void* g;                 // [tokens][g_ld]
   int64_t g_ld;
   // kProduct
-  const float* unscale;    // one factor on everything, or null
+  const float* unscale;    // one factor on everything
 };
 
 __host__ __device__ constexpr int stage_bytes(int bn, int cg, int am) { return (am + bn / cg) * kRowBytes; }
@@ -513,9 +513,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
     const int quarter = warp & 3;
     const int row_in_tile = static_cast<int>(cta_rank) * kBM + quarter * 32 + lane;
     float unscale = 1.0f;
-    if constexpr (MODE == kProduct) {
-      if (p.unscale != nullptr) unscale = __ldg(p.unscale);
-    }
+    if constexpr (MODE == kProduct) unscale = __ldg(p.unscale);
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int i = 0;; ++i) {

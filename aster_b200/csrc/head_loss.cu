@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <mutex>
 
 #include "common.h"
 #include "head_kernel.cuh"
@@ -77,6 +78,8 @@ __global__ void __launch_bounds__(256) teacher_kernel(const void* __restrict__ l
   __shared__ float s_t[kMaxTop];
   __shared__ float buf[32];
   const size_t row = blockIdx.x, base = row * top;
+  sm100::griddep_launch_dependents();
+  sm100::griddep_wait();
   float mx = -INFINITY, any = 0.0f, bad = 0.0f;
   for (int j = threadIdx.x; j < top; j += blockDim.x) {
     const long long id = load_index(ids_in, bits, base + j);
@@ -137,19 +140,24 @@ struct JoinParams {
   uint32_t* ticket;
 };
 
-// 32 rows per block: warp g joins every 32nd tile of all rows (coalesced), then warp r finishes row r.
-// The last block to finish adds the blocks' sums in their order, so that a repeated call gives the same bits.
-__global__ void __launch_bounds__(1024) join_kernel(const JoinParams p) {
-  __shared__ float s_m[32][33], s_s[32][33], s_z[32][33];
-  __shared__ float s_loss[32], s_kept[32];
+// 8 rows per block of 8 warps.  A thread joins every 32nd tile of one row (8 lanes read 8 neighbouring rows
+// of a tile, 64 bytes), then warp r finishes row r.  The last block to finish adds the blocks' sums in their
+// order, so that a repeated call gives the same bits.
+constexpr int kJoinRows = 8;
+constexpr int kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) {
+  __shared__ float s_m[32][kJoinRows + 1], s_s[32][kJoinRows + 1], s_z[32][kJoinRows + 1];
+  __shared__ float s_loss[kJoinRows], s_kept[kJoinRows];
   __shared__ uint32_t s_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  sm100::griddep_wait();
   {
-    const int row = blockIdx.x * 32 + lane;
+    const int r = threadIdx.x % kJoinRows, group = threadIdx.x / kJoinRows;
+    const int row = blockIdx.x * kJoinRows + r;
     float m = -INFINITY, s = 0.0f, z = 0.0f;
     if (row < p.tokens) {
 #pragma unroll 4
-      for (int n = warp; n < p.n_blocks; n += 32) {
+      for (int n = group; n < p.n_blocks; n += 32) {
         const float2 t = __ldcs(p.part + static_cast<size_t>(n) * p.tokens + row);
         const float nm = fmaxf(m, t.x);
         const float b = nm == -INFINITY ? 0.0f : nm;
@@ -158,12 +166,12 @@ __global__ void __launch_bounds__(1024) join_kernel(const JoinParams p) {
         if (p.part_z != nullptr) z += __ldcs(p.part_z + static_cast<size_t>(n) * p.tokens + row);
       }
     }
-    s_m[warp][lane] = m;
-    s_s[warp][lane] = s;
-    s_z[warp][lane] = z;
+    s_m[group][r] = m;
+    s_s[group][r] = s;
+    s_z[group][r] = z;
   }
   __syncthreads();
-  const int row = blockIdx.x * 32 + warp;
+  const int row = blockIdx.x * kJoinRows + warp;
   const float my_m = s_m[lane][warp];
   float m = my_m, s = s_s[lane][warp], z = s_z[lane][warp];
 #pragma unroll
@@ -212,18 +220,16 @@ __global__ void __launch_bounds__(1024) join_kernel(const JoinParams p) {
     s_kept[warp] = kept;
   }
   __syncthreads();
-  if (warp == 0) {
-    float a = s_loss[lane], k = s_kept[lane];
+  if (threadIdx.x == 0) {
+    float a = 0.0f, k = 0.0f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      k += __shfl_xor_sync(0xffffffffu, k, o);
+    for (int r = 0; r < kJoinRows; ++r) {
+      a += s_loss[r];
+      k += s_kept[r];
     }
-    if (lane == 0) {
-      p.block_sums[blockIdx.x] = make_float2(a, k);
-      __threadfence();
-      s_last = atomicAdd(p.ticket, 1u) == gridDim.x - 1 ? 1u : 0u;
-    }
+    p.block_sums[blockIdx.x] = make_float2(a, k);
+    __threadfence();
+    s_last = atomicAdd(p.ticket, 1u) == gridDim.x - 1 ? 1u : 0u;
   }
   __syncthreads();
   if (s_last == 0u) return;
@@ -239,7 +245,7 @@ __global__ void __launch_bounds__(1024) join_kernel(const JoinParams p) {
     a += __shfl_xor_sync(0xffffffffu, a, o);
     k += __shfl_xor_sync(0xffffffffu, k, o);
   }
-  __shared__ double d_a[32], d_k[32];
+  __shared__ double d_a[kJoinThreads / 32], d_k[kJoinThreads / 32];
   if (lane == 0) {
     d_a[warp] = a;
     d_k[warp] = k;
@@ -247,7 +253,7 @@ __global__ void __launch_bounds__(1024) join_kernel(const JoinParams p) {
   __syncthreads();
   if (threadIdx.x == 0) {
     a = k = 0.0;
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < kJoinThreads / 32; ++i) {
       a += d_a[i];
       k += d_k[i];
     }
@@ -257,14 +263,19 @@ __global__ void __launch_bounds__(1024) join_kernel(const JoinParams p) {
   }
 }
 
-// Row factors c_t = dL/dL_t * dL_t/d(softmax - labels), 0 for rows without a loss.  fp16: all of them
-// under one power of two that puts the largest at 2^13..2^14, so that G = c (softmax - labels) keeps
-// its digits down to 2^-38 of the largest factor; `unscale` takes it out of the gradients again, exactly.
+// Row factors c_t = dL/dL_t * dL_t/d(softmax - labels), 0 for rows without a loss, divided by the largest
+// of them: G = c_t (softmax - labels) is rounded to 16 bits, and with equal factors (mean, sum) its
+// entries at the labels are then close to 1 and -- nearly -- exact.  (Under the plain factor 1/N all of
+// them carried the one rounding error of 1/N: the gradients were off by 0.0035 instead of 0.0017, which
+// is the rounding of the result.)  fp16: the largest factor is 2^13, so that small probabilities keep
+// their digits, too.  `unscale` takes the divisor out of the gradients again, in fp32.
 __global__ void __launch_bounds__(1024) factor_kernel(const float* __restrict__ grad_loss, int per_row, const float* __restrict__ share, float row_scale,
                                                       const void* __restrict__ target, int index_bits, long long ignore_index, int vocab,
                                                       const float* __restrict__ weight, int tokens, int half_range, float* __restrict__ coef,
                                                       float* __restrict__ unscale) {
   __shared__ float buf[32];
+  sm100::griddep_launch_dependents();
+  sm100::griddep_wait();
   const float sh = *share;
   auto factor = [&](int t) -> float {
     float w;
@@ -276,23 +287,22 @@ __global__ void __launch_bounds__(1024) factor_kernel(const float* __restrict__ 
     }
     return w == 0.0f ? 0.0f : w * row_scale * (sh * grad_loss[per_row ? t : 0]);
   };
-  float scale = 1.0f;
-  if (half_range) {
-    float mx = 0.0f;
-    for (int t = threadIdx.x; t < tokens; t += blockDim.x) {
-      const float c = fabsf(factor(t));
-      if (c < INFINITY) mx = fmaxf(mx, c);
-    }
-    mx = block_reduce(mx, true, buf);
-    if (mx > 0.0f) scale = exp2f(static_cast<float>(max(-126, min(126, 13 - ilogbf(mx)))));
+  const float top = half_range ? 8192.0f : 1.0f;
+  float mx = 0.0f;
+  for (int t = threadIdx.x; t < tokens; t += blockDim.x) {
+    const float c = fabsf(factor(t));
+    if (c < INFINITY) mx = fmaxf(mx, c);
   }
-  for (int t = threadIdx.x; t < tokens; t += blockDim.x) coef[t] = factor(t) * scale;
-  if (threadIdx.x == 0) *unscale = 1.0f / scale;
+  mx = block_reduce(mx, true, buf);
+  if (mx == 0.0f) mx = 1.0f;
+  for (int t = threadIdx.x; t < tokens; t += blockDim.x) coef[t] = factor(t) / mx * top;
+  if (threadIdx.x == 0) *unscale = mx / top;
 }
 
 // dX = sum of its fp32 parts, in their order, rounded once.  n4 = elements / 4.
 template <typename T16>
 __global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ parts, int splits, size_t n4, T16* __restrict__ out) {
+  sm100::griddep_wait();
   for (size_t i = static_cast<size_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n4; i += static_cast<size_t>(gridDim.x) * blockDim.x) {
     float4 a = __ldcs(reinterpret_cast<const float4*>(parts) + i);
     for (int s = 1; s < splits; ++s) {
@@ -322,8 +332,9 @@ int ring(Tiling* t) {
 // CTA pairs (256-row tiles) unless single CTAs (128 rows) leave at least a fifth fewer padded rows.
 int choose_cg(int64_t tokens) { return div_up(tokens, 128) * 128 * 5 <= div_up(tokens, 256) * 256 * 4 ? 1 : 2; }
 
-// Tile of z: of the widths from 256 down, the one whose rounds of tiles cost least; a K block costs its
-// columns, but no less than 128 of them (the read of A), and a little that does not depend on the width.
+// Tile of z: of the widths from 256 down, the one whose rounds of tiles cost least.  A K block of a tile costs
+// what the L2 sends its SM, the rows of A and of B that a CTA stages: at 64 bytes a cycle that is 512 cycles
+// for a pair's 256 x 256, as long as its MMAs, and longer than them for everything narrower.
 Tiling z_tiling(int64_t tokens, int64_t cols) {
   Tiling t = {};
   t.cg = choose_cg(tokens);
@@ -331,7 +342,7 @@ Tiling z_tiling(int64_t tokens, int64_t cols) {
   const int64_t units = kSms / t.cg, m_blocks = div_up(tokens, 128 * t.cg);
   int64_t best = 0;
   for (int bn = 256; bn >= 64; bn -= 32) {
-    const int64_t cost = div_up(m_blocks * div_up(cols, bn), units) * (std::max(bn, 128) + 8);
+    const int64_t cost = div_up(m_blocks * div_up(cols, bn), units) * (t.am + bn / t.cg);
     if (t.bn == 0 || cost < best) {
       t.bn = bn;
       best = cost;
@@ -387,7 +398,7 @@ int make_plan(const b200_head_desc& d, Plan* p) {
   p->f_part_z = take(d.kind == B200_HEAD_CROSS_ENTROPY && d.label_smoothing > 0.0f ? static_cast<size_t>(p->n_blocks) * T * sizeof(float) : 0);
   p->f_label_z = take(T * top * sizeof(float));
   p->f_entropy = take(d.kind == B200_HEAD_DISTILL ? T * sizeof(float) : 0);
-  p->f_sums = take(static_cast<size_t>(div_up(d.tokens, 32)) * sizeof(float2));
+  p->f_sums = take(static_cast<size_t>(div_up(d.tokens, kJoinRows)) * sizeof(float2));
   p->f_ticket = take(sizeof(uint32_t));
   p->f_bytes = at;
   at = 0;
@@ -447,8 +458,49 @@ uint32_t idesc(int dtype, const Tiling& t, bool a_mn, bool b_mn) {
   return sm100::make_idesc(1u, f, f, static_cast<uint32_t>(head::kBM * t.cg), static_cast<uint32_t>(t.bn)) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
 }
 
+// What a device needs to be asked or told once: that it is an sm_100 part, the address of its status words,
+// and the kernels' shared-memory limit there.
+constexpr int kMaxDevices = 64;
+struct DeviceState {
+  std::once_flag once;
+  int rc = B200_OK;
+  char error[256] = {};
+  uint32_t* status = nullptr;
+};
+DeviceState g_devices[kMaxDevices];
+
+int init_device(int dev, DeviceState* st) {
+  int major = 0;
+  B200_CUDA_OK(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev));
+  if (major != 10) return b200::fail(B200_ERR_NO_DEVICE, "device %d has compute capability %d.x; the kernels need sm_100", dev, major);
+  for (int dtype : {B200_F16, B200_BF16}) {
+    for (int cg : {1, 2}) {
+      for (KernelFn fn : {kernel_for<head::kStats>(cg, dtype), kernel_for<head::kGrad>(cg, dtype), kernel_for<head::kProduct>(cg, dtype)}) {
+        B200_CUDA_OK(cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+      }
+    }
+  }
+  void* p = nullptr;
+  B200_CUDA_OK(cudaGetSymbolAddress(&p, g_status));
+  st->status = static_cast<uint32_t*>(p);
+  return B200_OK;
+}
+
+int current_device(DeviceState** out) {
+  int dev = 0;
+  B200_CUDA_OK(cudaGetDevice(&dev));
+  B200_REQUIRE(dev >= 0 && dev < kMaxDevices, "head_loss: device index %d", dev);
+  DeviceState& st = g_devices[dev];
+  std::call_once(st.once, [&] {
+    st.rc = init_device(dev, &st);
+    if (st.rc != B200_OK) std::snprintf(st.error, sizeof(st.error), "%s", b200_last_error());
+  });
+  if (st.rc != B200_OK) return b200::fail(st.rc, "%s", st.error);
+  *out = &st;
+  return B200_OK;
+}
+
 int launch(KernelFn fn, const Tiling& t, Params* p, const CUtensorMap (&maps)[4], cudaStream_t stream) {
-  B200_CUDA_OK(cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
   int64_t items = p->prob[0].items;
   if (p->num_probs > 1) items += p->prob[1].items;
   p->bn = t.bn;
@@ -475,6 +527,24 @@ int launch(KernelFn fn, const Tiling& t, Params* p, const CUtensorMap (&maps)[4]
   cfg.attrs = attr;
   cfg.numAttrs = n;
   B200_CUDA_OK(cudaLaunchKernelEx(&cfg, fn, maps[0], maps[1], maps[2], maps[3], *p));
+  b200::count_launch();
+  B200_CUDA_OK(cudaGetLastError());
+  return B200_OK;
+}
+
+// A small kernel that begins with griddep_wait: its launch overlaps the end of the kernel before it.
+template <typename... Args, typename... Actual>
+int launch_small(void (*fn)(Args...), unsigned grid, unsigned threads, cudaStream_t stream, Actual... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  B200_CUDA_OK(cudaLaunchKernelEx(&cfg, fn, static_cast<Args>(args)...));
   b200::count_launch();
   B200_CUDA_OK(cudaGetLastError());
   return B200_OK;
@@ -532,18 +602,14 @@ int common_checks(const b200_head_desc* desc, const void* x, const void* w, cons
                "head_loss: x, w, saved and workspace must be 16-byte aligned");
   B200_REQUIRE((reinterpret_cast<uintptr_t>(labels) & static_cast<uintptr_t>(desc->index_bits / 8 - 1)) == 0, "head_loss: labels must be aligned to their elements");
   if (workspace == nullptr || bytes < need) return b200::fail(B200_ERR_WORKSPACE, "head_loss: needs a %zu-byte workspace, got %zu", need, bytes);
-  int dev = 0, major = 0;
-  B200_CUDA_OK(cudaGetDevice(&dev));
-  B200_CUDA_OK(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev));
-  if (major != 10) return b200::fail(B200_ERR_NO_DEVICE, "device %d has compute capability %d.x; the kernels need sm_100", dev, major);
   return B200_OK;
 }
 
 int status_words(uint32_t** words) {
-  void* p = nullptr;
-  B200_CUDA_OK(cudaGetSymbolAddress(&p, g_status));
-  *words = static_cast<uint32_t*>(p);
-  return B200_OK;
+  DeviceState* st = nullptr;
+  const int rc = current_device(&st);
+  if (rc == B200_OK) *words = st->status;
+  return rc;
 }
 
 }  // namespace
@@ -583,13 +649,11 @@ int b200_head_loss_forward(const b200_head_desc* desc, const void* x, const void
   rc = status_words(&status);
   if (rc != B200_OK) return rc;
   if (d.kind == B200_HEAD_DISTILL) {
-    const int threads = d.top <= 32 ? 32 : (d.top <= 64 ? 64 : (d.top <= 128 ? 128 : 256));
-    teacher_kernel<<<static_cast<unsigned>(d.tokens), threads, 0, s>>>(teacher_logits, d.dtype_teacher, labels, d.index_bits, d.top, static_cast<int>(d.vocab),
-                                                                      1.0f / d.temperature, reinterpret_cast<int32_t*>(sv + pl.s_ids),
-                                                                      reinterpret_cast<float*>(sv + pl.s_probs), reinterpret_cast<float*>(sv + pl.s_weight),
-                                                                      reinterpret_cast<float*>(ws + pl.f_entropy));
-    b200::count_launch();
-    B200_CUDA_OK(cudaGetLastError());
+    const unsigned threads = d.top <= 32 ? 32u : (d.top <= 64 ? 64u : (d.top <= 128 ? 128u : 256u));
+    rc = launch_small(teacher_kernel, static_cast<unsigned>(d.tokens), threads, s, teacher_logits, d.dtype_teacher, labels, d.index_bits, d.top, static_cast<int>(d.vocab),
+                      1.0f / d.temperature, reinterpret_cast<int32_t*>(sv + pl.s_ids), reinterpret_cast<float*>(sv + pl.s_probs), reinterpret_cast<float*>(sv + pl.s_weight),
+                      reinterpret_cast<float*>(ws + pl.f_entropy));
+    if (rc != B200_OK) return rc;
   }
   Params p;
   set_labels(d, pl, labels, saved, status, &p);
@@ -635,10 +699,7 @@ int b200_head_loss_forward(const b200_head_desc* desc, const void* x, const void
   j.share = reinterpret_cast<float*>(sv);
   j.block_sums = reinterpret_cast<float2*>(ws + pl.f_sums);
   j.ticket = p.ticket;
-  join_kernel<<<static_cast<unsigned>(div_up(d.tokens, 32)), 1024, 0, s>>>(j);
-  b200::count_launch();
-  B200_CUDA_OK(cudaGetLastError());
-  return B200_OK;
+  return launch_small(join_kernel, static_cast<unsigned>(div_up(d.tokens, kJoinRows)), kJoinThreads, s, j);
 }
 
 int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const void* w, const void* labels, const float* lse, const void* saved,
@@ -663,11 +724,10 @@ int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const voi
   float* unscale = reinterpret_cast<float*>(ws + pl.b_unscale);
   float* parts = reinterpret_cast<float*>(ws + pl.b_parts);
   void* g = ws + pl.b_g;
-  factor_kernel<<<1, 1024, 0, s>>>(grad_loss, d.reduction == B200_REDUCE_NONE, reinterpret_cast<const float*>(sv), distill ? d.temperature : 1.0f, labels, d.index_bits,
-                                   d.ignore_index, static_cast<int>(d.vocab), distill ? reinterpret_cast<const float*>(sv + pl.s_weight) : nullptr,
-                                   static_cast<int>(d.tokens), d.dtype == B200_F16, coef, unscale);
-  b200::count_launch();
-  B200_CUDA_OK(cudaGetLastError());
+  rc = launch_small(factor_kernel, 1u, 1024u, s, grad_loss, d.reduction == B200_REDUCE_NONE, reinterpret_cast<const float*>(sv), distill ? d.temperature : 1.0f, labels,
+                    d.index_bits, d.ignore_index, static_cast<int>(d.vocab), distill ? reinterpret_cast<const float*>(sv + pl.s_weight) : nullptr,
+                    static_cast<int>(d.tokens), d.dtype == B200_F16, coef, unscale);
+  if (rc != B200_OK) return rc;
 
   CUtensorMap z_maps[4] = {};
   rc = b200::make_strided_operand_map(&z_maps[0], x, d.dtype, d.tokens, d.hidden, d.x_stride, static_cast<uint32_t>(pl.grad.am));
@@ -700,7 +760,7 @@ int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const voi
     Params q;
     std::memset(&q, 0, sizeof(q));
     q.status = status;
-    q.unscale = d.dtype == B200_F16 ? unscale : nullptr;
+    q.unscale = unscale;
     CUtensorMap maps[4] = {};
     if (grad_x != nullptr) {
       Problem& dx = q.prob[q.num_probs];
@@ -754,12 +814,9 @@ int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const voi
     const size_t n4 = static_cast<size_t>(d.tokens) * static_cast<size_t>(d.hidden) / 4;
     const unsigned blocks = static_cast<unsigned>(std::min<size_t>((n4 + 255) / 256, kSms * 8));
     if (d.dtype == B200_F16) {
-      sum_parts_kernel<__half><<<blocks, 256, 0, s>>>(parts, pl.splits, n4, static_cast<__half*>(grad_x));
-    } else {
-      sum_parts_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(parts, pl.splits, n4, static_cast<__nv_bfloat16*>(grad_x));
+      return launch_small(sum_parts_kernel<__half>, blocks, 256u, s, parts, pl.splits, n4, static_cast<__half*>(grad_x));
     }
-    b200::count_launch();
-    B200_CUDA_OK(cudaGetLastError());
+    return launch_small(sum_parts_kernel<__nv_bfloat16>, blocks, 256u, s, parts, pl.splits, n4, static_cast<__nv_bfloat16*>(grad_x));
   }
   return B200_OK;
 }

@@ -18,12 +18,14 @@ storage to ``b200_head_loss_*``; torch's current stream is used, there is no CPU
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import weakref
 from typing import Optional, Sequence
 
 import torch
 
 from . import _native as nat
-from .torch_op import _on_device, _raw_stream
+from .torch_op import _call, _raw_stream
 
 _DTYPES = {torch.bfloat16: nat.BF16, torch.float16: nat.F16}
 _TEACHER_DTYPES = {torch.float32: nat.F32, torch.bfloat16: nat.BF16, torch.float16: nat.F16}
@@ -34,7 +36,8 @@ MAX_TOP = 1024  # teacher entries per row
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """Two dimensions, the last one contiguous, rows a multiple of 16 bytes apart and aligned (else a copy)."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     if t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1])):
         t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
@@ -74,6 +77,12 @@ def _sizes(d: nat.HeadDesc) -> nat.HeadSizes:
     return s
 
 
+@functools.lru_cache(maxsize=256)
+def _sizes_of(fields: bytes) -> nat.HeadSizes:
+    """The sizes follow from the description alone."""
+    return _sizes(nat.HeadDesc.from_buffer_copy(fields))
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -92,17 +101,17 @@ class _Head:
 
     def forward(self):
         dev, tokens = self.x.device, self.x.shape[0]
-        f32 = dict(dtype=torch.float32, device=dev)
         if tokens == 0:  # nothing to launch
-            loss = torch.empty(0, **f32) if self.per_row else torch.full((), float("nan") if self.desc.reduction == nat.REDUCE_MEAN else 0.0, **f32)
-            return loss, torch.empty(0, **f32), torch.empty(0, dtype=torch.uint8, device=dev)
-        sizes = _sizes(self.desc)
-        loss = torch.empty(tokens if self.per_row else (), **f32)
-        lse = torch.empty(tokens, **f32)
-        saved = torch.empty(sizes.saved, dtype=torch.uint8, device=dev)
-        ws = torch.empty(sizes.forward_workspace, dtype=torch.uint8, device=dev)
-        _on_device(dev, lambda: nat.call("b200_head_loss_forward", C.byref(self.desc), self.x.data_ptr(), self.w.data_ptr(), self.labels.data_ptr(),
-                                         _ptr(self.teacher), loss.data_ptr(), lse.data_ptr(), saved.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(dev)))
+            none = self.x.new_empty(0, dtype=torch.float32)
+            loss = none if self.per_row else self.x.new_full((), float("nan") if self.desc.reduction == nat.REDUCE_MEAN else 0.0, dtype=torch.float32)
+            return loss, none.clone(), self.x.new_empty(0, dtype=torch.uint8)
+        sizes = _sizes_of(bytes(self.desc))
+        loss = self.x.new_empty(tokens if self.per_row else (), dtype=torch.float32)
+        lse = self.x.new_empty(tokens, dtype=torch.float32)
+        saved = self.x.new_empty(sizes.saved, dtype=torch.uint8)
+        ws = self.x.new_empty(sizes.forward_workspace, dtype=torch.uint8)
+        _call(dev, nat.lib().b200_head_loss_forward, C.byref(self.desc), self.x.data_ptr(), self.w.data_ptr(), self.labels.data_ptr(), _ptr(self.teacher),
+              loss.data_ptr(), lse.data_ptr(), saved.data_ptr(), ws.data_ptr(), sizes.forward_workspace)
         return loss, lse, saved
 
     def backward(self, grad, lse, saved, want_x: bool, want_w: bool):
@@ -111,10 +120,12 @@ class _Head:
         if tokens == 0:
             return dx, torch.zeros(self.w.shape, dtype=self.w.dtype, device=dev) if want_w else None
         dw = torch.empty(self.w.shape, dtype=self.w.dtype, device=dev) if want_w else None
-        grad = grad.to(torch.float32).contiguous()
-        ws = torch.empty(_sizes(self.desc).backward_workspace, dtype=torch.uint8, device=dev)
-        _on_device(dev, lambda: nat.call("b200_head_loss_backward", C.byref(self.desc), self.x.data_ptr(), self.w.data_ptr(), self.labels.data_ptr(),
-                                         lse.data_ptr(), saved.data_ptr(), grad.data_ptr(), _ptr(dx), _ptr(dw), ws.data_ptr(), ws.numel(), _raw_stream(dev)))
+        if grad.dtype != torch.float32 or not grad.is_contiguous():
+            grad = grad.to(torch.float32).contiguous()
+        need = _sizes_of(bytes(self.desc)).backward_workspace
+        ws = self.x.new_empty(need, dtype=torch.uint8)
+        _call(dev, nat.lib().b200_head_loss_backward, C.byref(self.desc), self.x.data_ptr(), self.w.data_ptr(), self.labels.data_ptr(), lse.data_ptr(),
+              saved.data_ptr(), grad.data_ptr(), _ptr(dx), _ptr(dw), ws.data_ptr(), need)
         return dx, dw
 
 
@@ -142,31 +153,35 @@ def _distill_head(x, w, teacher_logits, teacher_ids, temperature, reduction, gra
     return _Head(x, w, teacher_ids, reduction, kind=nat.HEAD_DISTILL, temperature=temperature, teacher=teacher_logits, grad_bytes=grad_bytes)
 
 
-_STREAM_NOTE = "aster_b200.stream"
+# Graphs of these functions that were made on a default stream, each with its leaves, for as long as they live.
+# Autograd keeps one accumulation node per leaf, tied to the stream that was current when it was made, while any
+# graph refers to it.  A backward pass that is being captured cannot join the default stream, so a graph left
+# over from there would break the capture (and, from the engine's own threads, the process): such a capture is
+# refused before it begins.
+_default_stream_graphs: dict = {}
 
 
-def _note_leaves(*tensors: torch.Tensor) -> list:
-    """Autograd keeps one accumulation node per leaf, tied to the stream that was current when it was made,
-    for as long as any graph refers to it.  A backward pass that is being captured cannot join the default
-    stream, so a graph left over from there would break the capture (and, from the engine's own threads, the
-    process).  The node remembers its stream here, and such a capture is refused before it begins.  The
-    caller holds the returned nodes until its own graph refers to them."""
-    nodes = []
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t.requires_grad and t.is_leaf:
-                node = torch.autograd.graph.get_gradient_edge(t).node
-                stream = torch.cuda.current_stream(t.device).cuda_stream
-                if node.metadata.setdefault(_STREAM_NOTE, stream) == 0 and stream != 0 and torch.cuda.is_current_stream_capturing():
-                    raise RuntimeError("an autograd graph of the same leaf, made on the default stream, is still alive: its backward pass cannot be "
-                                       "captured; free that graph (delete its loss) before the capture")
-                nodes.append(node)
-    return nodes
+def _refuse_capture_beside(*tensors: torch.Tensor) -> None:
+    for leaves, _ in list(_default_stream_graphs.values()):
+        if any(ref() is t for ref in leaves for t in tensors):
+            raise RuntimeError("an autograd graph of the same leaf, made on the default stream, is still alive: a backward pass cannot be captured "
+                               "beside it; free that graph (delete its loss) before the capture")
+
+
+def _note_graph(ctx, x: torch.Tensor, w: torch.Tensor) -> None:
+    leaves = tuple(weakref.ref(t) for t in (x, w) if t.requires_grad and t.is_leaf)
+    if leaves:
+        key = id(ctx)
+        _default_stream_graphs[key] = (leaves, weakref.ref(ctx, lambda _: _default_stream_graphs.pop(key, None)))
 
 
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, head, shape):
+        if not _raw_stream(x.device):
+            _note_graph(ctx, x, w)
+        elif torch.cuda.is_current_stream_capturing():
+            _refuse_capture_beside(x, w)
         loss, lse, saved = head.forward()
         # the tensors come back through save_for_backward: it notices a change in place before the backward pass
         ctx.save_for_backward(x, w, head.labels, lse, saved)
@@ -195,10 +210,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     "mean" divides by the number of targets that count (NaN without any).  ``grad_bytes`` limits what the
     backward pass keeps of ``dL/dz`` at a time (0: 256 MiB)."""
     head = _xent_head(x, weight, target, ignore_index, label_smoothing, reduction, grad_bytes)
-    leaves = _note_leaves(x, weight)
-    loss = _HeadLoss.apply(x, weight, head, target.shape)
-    del leaves
-    return loss
+    return _HeadLoss.apply(x, weight, head, target.shape)
 
 
 def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor, *, temperature: float = 1.0,
@@ -212,10 +224,7 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: t
     nothing left have no loss and no gradient and do not count for "mean".  An id listed twice counts twice; an
     id beyond the vocabulary, or a logit that is NaN or plus infinity, makes the row NaN."""
     head = _distill_head(x, weight, teacher_logits, teacher_ids, temperature, reduction, grad_bytes)
-    leaves = _note_leaves(x, weight)
-    loss = _HeadLoss.apply(x, weight, head, teacher_ids.shape[:-1])
-    del leaves
-    return loss
+    return _HeadLoss.apply(x, weight, head, teacher_ids.shape[:-1])
 
 
 def head_loss_status() -> Sequence[int]:

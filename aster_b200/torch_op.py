@@ -64,11 +64,13 @@ def _gemm_run():
     return _run_fn
 
 
+_raw_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _raw_stream(device: torch.device) -> int:
     """Handle of torch's current stream on ``device`` (0 = the default stream)."""
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    if raw is not None:
-        return raw(device.index) or None
+    if _raw_stream_of is not None:
+        return _raw_stream_of(device.index) or None
     return torch.cuda.current_stream(device).cuda_stream or None
 
 
@@ -141,20 +143,22 @@ _MX_VALUE_DTYPES = {torch.float32: nat.F32, torch.bfloat16: nat.BF16, torch.floa
 _mx_lock = threading.Lock()
 
 
-def _on_device(device: torch.device, launch) -> None:
-    """Run ``launch`` with ``device`` current (the C ABI works on the current device, like torch)."""
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
-    def ready() -> None:
-        if device.index not in _ready_devices:
-            nat.init_current()
-            _ready_devices.add(device.index)
-        launch()
 
-    if torch.cuda.current_device() == device.index:
-        ready()
+def _call(device: torch.device, fn, *args) -> None:
+    """``fn(*args, stream)`` with torch's current stream of ``device``, with ``device`` current (the C ABI
+    works on the current device, like torch)."""
+    if device.index in _ready_devices and _current_device() == device.index:
+        status = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            ready()
+            if device.index not in _ready_devices:
+                nat.init_current()
+                _ready_devices.add(device.index)
+            status = fn(*args, _raw_stream(device))
+    if status != nat.OK:
+        nat.check(status)
 
 
 def _mx_scales_bytes(rows: int, K: int) -> int:
@@ -164,6 +168,10 @@ def _mx_scales_bytes(rows: int, K: int) -> int:
 
 def _check_mx_operand(name: str, q: torch.Tensor, scales: torch.Tensor) -> None:
     """Packed codes ``[rows, K/2]`` and their scales, in the layout that ``quantize_mx`` returns."""
+    if q.is_cuda and q.dtype is torch.uint8 and scales.dtype is torch.uint8 and q.dim() == 2 and scales.dim() == 1 and scales.device == q.device:
+        rows, half = q.shape
+        if rows >= 1 and half >= 16 and half % 16 == 0 and scales.shape[0] == _mx_scales_bytes(rows, 2 * half):
+            return
     for what, t in ((name, q), (f"{name}'s scales", scales)):
         if not t.is_cuda:
             raise RuntimeError(f"{what} must be a CUDA tensor (there is no CPU path)")
@@ -178,7 +186,8 @@ def _check_mx_operand(name: str, q: torch.Tensor, scales: torch.Tensor) -> None:
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """Contiguous and 16-byte aligned (a view can start anywhere)."""
-    t = t.contiguous()
+    if not t.is_contiguous():
+        return t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -197,10 +206,9 @@ def quantize_mx_direct(x: torch.Tensor, elem: str = "e2m1") -> tuple[torch.Tenso
     M, K = x.shape
     if x.stride(1) != 1 or (M > 1 and x.stride(0) < K):
         x = x.contiguous()
-    q = torch.empty((M, K // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(_mx_scales_bytes(M, K), dtype=torch.uint8, device=x.device)
-    _on_device(x.device, lambda: nat.check(nat.lib().b200_quantize_mx(
-        x.data_ptr(), _MX_VALUE_DTYPES[x.dtype], M, K, x.stride(0), nat.MXE2M1, q.data_ptr(), scales.data_ptr(), _raw_stream(x.device))))
+    q = x.new_empty((M, K // 2), dtype=torch.uint8)
+    scales = x.new_empty(_mx_scales_bytes(M, K), dtype=torch.uint8)
+    _call(x.device, nat.lib().b200_quantize_mx, x.data_ptr(), _MX_VALUE_DTYPES[x.dtype], M, K, x.stride(0), nat.MXE2M1, q.data_ptr(), scales.data_ptr())
     return q, scales
 
 
@@ -211,9 +219,8 @@ def dequantize_mx_direct(q: torch.Tensor, scales: torch.Tensor, out_dtype: torch
         raise RuntimeError(f"unsupported out_dtype {out_dtype}")
     q, scales = _aligned(q), _aligned(scales)
     M, K = q.shape[0], 2 * q.shape[1]
-    out = torch.empty((M, K), dtype=out_dtype, device=q.device)
-    _on_device(q.device, lambda: nat.check(nat.lib().b200_dequantize_mx(
-        q.data_ptr(), scales.data_ptr(), nat.MXE2M1, M, K, _MX_VALUE_DTYPES[out_dtype], out.data_ptr(), _raw_stream(q.device))))
+    out = q.new_empty((M, K), dtype=out_dtype)
+    _call(q.device, nat.lib().b200_dequantize_mx, q.data_ptr(), scales.data_ptr(), nat.MXE2M1, M, K, _MX_VALUE_DTYPES[out_dtype], out.data_ptr())
     return out
 
 
@@ -233,21 +240,25 @@ def gemm_mx_nt_direct(a: torch.Tensor, scales_a: torch.Tensor, b: torch.Tensor, 
         raise RuntimeError(f"bias must be {N} float32 values on {a.device}")
     a, scales_a, b, scales_b = _aligned(a), _aligned(scales_a), _aligned(b), _aligned(scales_b)
     bias = None if bias is None else bias.contiguous()
-    device = a.device
-    out = torch.empty((M, N), dtype=out_dtype, device=device)
-
-    def launch() -> None:
-        with _mx_lock:
-            key = (device.index, M, N, K, "mxe2m1", _OUT_DTYPES[out_dtype], _EPILOGUES[(bias is not None, relu)])
-            if key not in _plans:
-                _plans[key] = (GemmPlan(*key[1:6], epilogue=key[6]), None)
-            plan = _plans[key][0]
-            nat.check(nat.lib().b200_gemm_plan_set_mx_scales(plan.handle, scales_a.data_ptr(), scales_b.data_ptr()))
-            nat.check(_gemm_run()(plan.handle, a.data_ptr(), b.data_ptr(), out.data_ptr(), None if bias is None else bias.data_ptr(),
-                                  None, None, None, 0, _raw_stream(device)))
-
-    _on_device(device, launch)
+    out = a.new_empty((M, N), dtype=out_dtype)
+    _call(a.device, _gemm_mx, a, scales_a, b, scales_b, bias, relu, out)
     return out
+
+
+def _gemm_mx(a, scales_a, b, scales_b, bias, relu, out, stream) -> int:
+    M, N = out.shape
+    K = 2 * a.shape[1]
+    lib = nat.lib()
+    with _mx_lock:
+        key = (a.device.index, M, N, K, "mxe2m1", _OUT_DTYPES[out.dtype], _EPILOGUES[(bias is not None, relu)])
+        hit = _plans.get(key)
+        if hit is None:
+            hit = _plans[key] = (GemmPlan(*key[1:6], epilogue=key[6]), None)
+        handle = hit[0].handle
+        status = lib.b200_gemm_plan_set_mx_scales(handle, scales_a.data_ptr(), scales_b.data_ptr())
+        if status == nat.OK:
+            status = lib.b200_gemm_run(handle, a.data_ptr(), b.data_ptr(), out.data_ptr(), None if bias is None else bias.data_ptr(), None, None, None, 0, stream)
+    return status
 
 
 @torch.library.custom_op("aster_b200::quantize_mx", mutates_args=())
