@@ -149,7 +149,11 @@ enum : int { kMxNone = 0, kMx8 = 1, kMx4 = 2 };
 constexpr int kMx4StageElems = 256;  // elements of K in a 128-byte row of 4-bit elements
 // Scale blocks of one stage per 128 rows: 128 bytes of K are 4 blocks of 32 fp8 or 8 of fp4.
 __host__ __device__ constexpr int scale_blocks_per_rows(int mx) { return mx == kMx4 ? 2 : 1; }
-__host__ __device__ constexpr int scale_load_bytes(int bn, int mx) { return mx == kMxNone ? 0 : kScaleBlockBytes * scale_blocks_per_rows(mx) * (1 + bn / 128); }
+// 128-row groups of B that a tile touches.  64- and 192-column tiles start in the middle of a group every
+// other time: 192 columns are then the last half of one and all of the next, else all of one and the first
+// half of the next.
+__host__ __device__ constexpr int scale_groups_b(int bn) { return (bn + 127) / 128; }
+__host__ __device__ constexpr int scale_load_bytes(int bn, int mx) { return mx == kMxNone ? 0 : kScaleBlockBytes * scale_blocks_per_rows(mx) * (1 + scale_groups_b(bn)); }
 __host__ __device__ constexpr int scale_stage_bytes(int bn, int mx) { return (scale_load_bytes(bn, mx) + 1023) / 1024 * 1024; }
 // `am` = rows of A that a stage holds: 128, or 32 / 64 for skinny problems (M <= am), whose
 // stages then spend their bytes on B.  The MMA still reads 128 rows from the stage's start; the
@@ -168,12 +172,17 @@ constexpr int kBarrierBytes = 384;
 __host__ __device__ constexpr int a_overrun_bytes(int bn, int cg = 1, int mx = kMxNone, int am = kBM) {
   return kBM * kRowBytes > stage_bytes(bn, cg, mx, am) ? kBM * kRowBytes - stage_bytes(bn, cg, mx, am) : 0;
 }
+// Shared memory in which an epilogue warp turns 32 rows x 128 bytes of C around (4-bit operands, full tiles).
+constexpr int kCStoreBytes = 32 * 128;
+__host__ __device__ constexpr int c_store_bytes(int mx, int am) {
+  return mx == kMx4 && am == kBM ? kEpilogueWarps * kCStoreBytes : 0;
+}
 __host__ __device__ constexpr int smem_bytes(int bn, int stages, int cg = 1, int mx = kMxNone, int am = kBM) {
-  return stages * stage_bytes(bn, cg, mx, am) + a_overrun_bytes(bn, cg, mx, am) + kBarrierBytes + 1024;
+  return stages * stage_bytes(bn, cg, mx, am) + c_store_bytes(mx, am) + a_overrun_bytes(bn, cg, mx, am) + kBarrierBytes + 1024;
 }
 // Two accumulators of bn columns; a block-scaled kernel adds two sets of 16 (fp8) or 24 (fp4) scale columns.
 __host__ __device__ constexpr int scale_tmem_cols(int mx) { return mx == kMx4 ? 24 : 16; }
-__host__ __device__ constexpr int tmem_columns(int bn, int mx = kMxNone) {  // bn is a power of two
+__host__ __device__ constexpr int tmem_columns(int bn, int mx = kMxNone) {  // a power of two
   return mx != kMxNone ? 512 : (2 * bn < 32 ? 32 : 2 * bn);
 }
 
@@ -437,10 +446,10 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                const __grid_constant__ CUtensorMap tmap_sfa, const __grid_constant__ CUtensorMap tmap_sfb, const Params p) {
 #if defined(__CUDA_ARCH_FEAT_SM100_ALL)
   using namespace sm100;
-  static_assert(BN == 32 || BN == 64 || BN == 128 || BN == 256, "unsupported tile width");
+  static_assert(BN == 32 || BN == 64 || BN == 128 || BN == 256 || (BN == 192 && MX == kMx4 && CG == 2), "unsupported tile width");
   static_assert(CG == 1 || CG == 2, "one CTA or a CTA pair");
   constexpr uint32_t kBRows = BN / CG;  // B rows staged by this CTA
-  static_assert(AM == kBM || (CG == 1 && MX == kMxNone && (AM == 32 || AM == 64)), "short A stages: one CTA, plain operands, 32 or 64 rows");
+  static_assert(AM == kBM || (CG == 1 && MX != kMx8 && (AM == 32 || AM == 64)), "short A stages: one CTA, plain or 4-bit operands, 32 or 64 rows");
   constexpr uint32_t kABytes = AM * kRowBytes;
   constexpr uint32_t kBBytes = kBRows * kRowBytes;
   constexpr uint32_t kStageBytes = stage_bytes(BN, CG, MX, AM);
@@ -450,14 +459,16 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   // 512 TMEM columns and leave none for the scales (the epilogue then does not overlap the next
   // main loop, which costs less than the shared-memory bound of a 128-column tile).
   constexpr int kAccBufs = (MX != kMxNone && BN == 256) ? 1 : 2;
-  static_assert(MX == kMxNone || BN == 128 || BN == 256, "block-scaled tiles are 128 or 256 columns wide");
+  static_assert(MX == kMxNone || BN == 128 || BN == 256 || (MX == kMx4 && (BN == 192 || BN == 64)), "block-scaled tiles are 128 or 256 columns wide, with fp4 also 64 and 192");
   static_assert(MX == kMxNone || kAccBufs * BN + 2 * scale_tmem_cols(MX) <= 512, "accumulators and scales share the 512 columns");
   constexpr int kTileM = kBM * CG;
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_raw_u32 = smem_u32(smem_raw);
   const uint32_t smem_base = (smem_raw_u32 + 1023u) & ~1023u;  // swizzled tiles need 1024-byte alignment
-  const uint32_t bar_base = smem_base + static_cast<uint32_t>(p.stages) * kStageBytes + a_overrun_bytes(BN, CG, MX, AM);
+  constexpr bool kWholeTile = c_store_bytes(MX, AM) != 0;
+  [[maybe_unused]] const uint32_t c_smem = smem_base + static_cast<uint32_t>(p.stages) * kStageBytes;  // turn-around buffers of the epilogue
+  const uint32_t bar_base = c_smem + static_cast<uint32_t>(c_store_bytes(MX, AM)) + a_overrun_bytes(BN, CG, MX, AM);
   uint8_t* bar_ptr = smem_raw + (bar_base - smem_raw_u32);
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 128u + 8u * s; };
@@ -628,7 +639,7 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           constexpr int kSfBlocks = scale_blocks_per_rows(MX);
           [[maybe_unused]] const int ks = kSfBlocks == 1 ? min(kb0 + kb, p.sf_k_stages - 1) : kSfBlocks * (kb0 + kb);
           [[maybe_unused]] const int sfa_blk = m_blk * CG + static_cast<int>(cta_rank);
-          [[maybe_unused]] const int sfb_blk = n_blk * (BN / 128);
+          [[maybe_unused]] const int sfb_blk = n_blk * BN / 128;
           if (p.debug_mode & 8) {
             // injected fault: the stage is never handed over, so the consumer's wait must run out
           } else if (kBringup && (p.debug_mode & 3) == 1) {
@@ -638,7 +649,7 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             if constexpr (MX != kMxNone) {
               tma_load_2d(sf_dst, &tmap_sfa, full_bar(stage), 0, sfa_blk * p.sf_k_stages + ks);
 #pragma unroll
-              for (int q = 0; q < BN / 128; ++q) {
+              for (int q = 0; q < scale_groups_b(BN); ++q) {
                 tma_load_2d(sf_dst + (1 + q) * kSfBlocks * kScaleBlockBytes, &tmap_sfb, full_bar(stage), 0, (sfb_blk + q) * p.sf_k_stages + ks);
               }
             }
@@ -652,7 +663,7 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             if constexpr (MX != kMxNone) {
               tma_load_2d_pair(sf_dst, &tmap_sfa, leader_full, 0, sfa_blk * p.sf_k_stages + ks);
 #pragma unroll
-              for (int q = 0; q < BN / 128; ++q) {
+              for (int q = 0; q < scale_groups_b(BN); ++q) {
                 tma_load_2d_pair(sf_dst + (1 + q) * kSfBlocks * kScaleBlockBytes, &tmap_sfb, leader_full, 0, (sfb_blk + q) * p.sf_k_stages + ks);
               }
             }
@@ -704,6 +715,13 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         const WorkItem w = decode_item(p, item);
         const int tile = w.tile;
         const int num_kb = w.nkb;
+        // Columns of TMEM (32 scales of B each) before the tile's first one in its first scale group.
+        [[maybe_unused]] uint32_t sfb_shift = 0;
+        if constexpr (BN % 128 != 0) {
+          int m_unused, n_blk;
+          tile_coords(p, tile, m_unused, n_blk);
+          sfb_shift = (n_blk & 1) != 0 ? 2u : 0u;
+        }
         if (!waiter.wait(acc_empty_bar(acc), acc_phase ^ 1u, kStatusMmaAccEmptyWait, tile, 0)) {
           ok = false;
           break;
@@ -729,8 +747,8 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
               if constexpr (MX == kMx4) {
                 const int left = p.K - (w.kb0 + kb) * kMx4StageElems;  // elements of K from this stage on
                 const uint32_t mmas = static_cast<uint32_t>(min(left + 63, kMx4StageElems) >> 6);
-                if (do_mma) umma_mx4_stage<CG, BN / 128>(tmem_d, a_lo, a_lo + b_off, desc_hi, idesc, kb != 0 ? 1u : 0u, sf_tmem, smem_desc_lo_scales(sf_smem), mmas);
-              } else if (do_mma) umma_mx_stage<CG, BN / 128>(tmem_d, a_lo, a_lo + b_off, desc_hi, idesc, kb != 0 ? 1u : 0u, sf_tmem, smem_desc_lo_scales(sf_smem));
+                if (do_mma) umma_mx4_stage<CG, scale_groups_b(BN)>(tmem_d, a_lo, a_lo + b_off, desc_hi, idesc, kb != 0 ? 1u : 0u, sf_tmem, smem_desc_lo_scales(sf_smem), mmas, sfb_shift);
+              } else if (do_mma) umma_mx_stage<CG, scale_groups_b(BN)>(tmem_d, a_lo, a_lo + b_off, desc_hi, idesc, kb != 0 ? 1u : 0u, sf_tmem, smem_desc_lo_scales(sf_smem));
             } else {
               if (do_mma) umma_stage<CG>(tmem_d, a_lo, a_lo + b_off, desc_hi, idesc, kb != 0 ? 1u : 0u, mma_kind);
             }
@@ -798,9 +816,9 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       const int split = w.split;
       int m_blk, n_blk;
       tile_coords(p, tile, m_blk, n_blk);
-      // A CTA with a single work item has no later main loop for this wait to hide behind: poll
+      // A CTA with a single work item (or accumulator) has no later main loop for this wait to hide behind: poll
       // tightly there (the launch ends with this epilogue); otherwise sleep between polls.
-      if (!waiter.wait_relaxed(acc_full_bar(acc), acc_phase, kStatusEpilogueAccFullWait, tile, num_items <= item_stride ? 20u : 256u)) {
+      if (!waiter.wait_relaxed(acc_full_bar(acc), acc_phase, kStatusEpilogueAccFullWait, tile, (kAccBufs == 1 || num_items <= item_stride) ? 20u : 256u)) {
         ok = false;
         break;
       }
@@ -911,12 +929,108 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 #pragma unroll
         for (int j = 0; j < 8; ++j) ahead[j] = partial(first_other, lo, j);
       }
+      // 4-bit operands shorten the main loop until the epilogue decides.  Whole tiles leave as whole 128-byte
+      // lines, turned around in 4 KB of shared memory per warp (a lane per row writes a piece of 128 bytes,
+      // eight lanes per row read it), because 32-byte stores to 32 rows cost more issue slots than all else
+      // here, and the accumulator goes back as soon as its last columns are in registers.  (Stores by
+      // TMA instead queue up behind the loads of the ring and were no faster.)
+      bool released = false;
+      if constexpr (kWholeTile) {
+        if (!tail_item && p.split_k <= 1 && n_vec_ok && !bringup_mode(p, 32 | 64)) {
+          constexpr int kCols = 128 / static_cast<int>(sizeof(OutT));  // columns per piece
+          const int n_cols = slab_ok ? min(BN, p.N - n_blk * BN) : 0;
+          const uint32_t buf = c_smem + static_cast<uint32_t>(quarter) * kCStoreBytes;
+          const uint32_t wr = buf + static_cast<uint32_t>(lane) * 128u;
+          const uint32_t wr_swz = static_cast<uint32_t>(lane & 7) << 4;
+          const int rd_row = lane >> 3, rd_chunk = lane & 7;  // of every 4 rows
+          const int row0 = m_blk * kTileM + static_cast<int>(cta_rank) * kBM + quarter * 32;
+#pragma unroll 1
+          for (int c = 0; c < n_cols; c += kCols) {
+            uint32_t v[kCols];
+            if constexpr (kCols == 64) {
+              tmem_ld_32x32b_x64(taddr + static_cast<uint32_t>(c), v);
+            } else {
+              tmem_ld_32x32b_x32(taddr + static_cast<uint32_t>(c), v);
+            }
+            tmem_ld_wait();
+            if (c + kCols >= n_cols) {
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) {
+                if constexpr (CG == 1) {
+                  mbar_arrive(acc_empty_bar(acc));
+                } else {
+                  mbar_arrive_remote(map_to_cta(acc_empty_bar(acc), 0u));
+                }
+              }
+              released = true;
+            }
+            const int col0 = n_blk * BN + c;
+            float x[kCols];
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) x[j] = __uint_as_float(v[j]);
+            if (alpha != 1.0f) {
+#pragma unroll
+              for (int j = 0; j < kCols; ++j) x[j] *= alpha;
+            }
+            if (p.bias != nullptr) {
+              if (p.bias_axis != 0) {
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) x[j] += bias_row;
+              } else if (col0 + kCols <= p.N && bias_vec_ok) {
+                const float4* b4 = reinterpret_cast<const float4*>(p.bias + col0);
+#pragma unroll
+                for (int j = 0; j < kCols / 4; ++j) {
+                  const float4 t = __ldg(b4 + j);
+                  x[4 * j] += t.x;
+                  x[4 * j + 1] += t.y;
+                  x[4 * j + 2] += t.z;
+                  x[4 * j + 3] += t.w;
+                }
+              } else {
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) x[j] += col0 + j < p.N ? __ldg(p.bias + col0 + j) : 0.0f;
+              }
+            }
+            if (p.relu) {
+#pragma unroll
+              for (int j = 0; j < kCols; ++j) x[j] = fmaxf(x[j], 0.0f);
+            }
+            __syncwarp();  // the previous piece has been read
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint32_t w4[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if constexpr (sizeof(OutT) == 4) {
+                  w4[e] = __float_as_uint(x[4 * j + e]);
+                } else {
+                  const __nv_bfloat162 t = __floats2bfloat162_rn(x[8 * j + 2 * e], x[8 * j + 2 * e + 1]);
+                  w4[e] = *reinterpret_cast<const uint32_t*>(&t);
+                }
+              }
+              st_shared_u4(wr + ((static_cast<uint32_t>(j) << 4) ^ wr_swz), w4[0], w4[1], w4[2], w4[3]);
+            }
+            __syncwarp();
+            const int col = col0 + rd_chunk * (kCols / 8);
+            OutT* dst = C + static_cast<size_t>(row0 + rd_row) * p.N + col;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = 4 * i + rd_row;
+              const uint4 t = ld_shared_u4(buf + static_cast<uint32_t>(r) * 128u + ((static_cast<uint32_t>(rd_chunk) ^ static_cast<uint32_t>(r & 7)) << 4));
+              if (row0 + r < p.M && col < p.N) *reinterpret_cast<uint4*>(dst) = t;  // a 16-byte piece exists or does not
+              dst += static_cast<size_t>(4) * p.N;
+            }
+          }
+          lo = hi;  // nothing left for the loops below; a slab without rows is handed back there
+        }
+      }
       // Whole tiles of a floating-point product (no K split of any kind, at least 64 columns) take
       // a leaner path: 64 columns per TMEM load and wait, i.e. two independent conversion and
       // store chains per iteration and half the loop trips.  An epilogue warp is a serial chain
       // on one scheduler; this is the cheap way to give it instruction-level parallelism.
       if constexpr (BN >= 64) {
-        if (!tail_item && p.split_k <= 1 && p.acc_int == 0 && !bringup_mode(p, 64)) {
+        if (!released && !tail_item && p.split_k <= 1 && p.acc_int == 0 && !bringup_mode(p, 64)) {
 #pragma unroll 1
           for (int c = 0; c < (slab_ok ? BN : 0); c += 64) {
             uint32_t v[64];
@@ -1076,7 +1190,7 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       }
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) {
+      if (lane == 0 && !released) {
         if constexpr (CG == 1) {
           mbar_arrive(acc_empty_bar(acc));
         } else {

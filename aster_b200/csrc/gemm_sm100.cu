@@ -124,10 +124,21 @@ KernelFn select_kernel_mx(int bn, bool f32, int cta_group) {
   return f32 ? gemm::gemm_tn_kernel<128, float, 1, MX> : gemm::gemm_tn_kernel<128, __nv_bfloat16, 1, MX>;
 }
 
+// 4-bit operands, one CTA, 64 columns or short A stages.
+template <int AM>
+KernelFn select_kernel_mx4_skinny(int bn, bool f32) {
+  if (bn == 64) return f32 ? gemm::gemm_tn_kernel<64, float, 1, gemm::kMx4, AM> : gemm::gemm_tn_kernel<64, __nv_bfloat16, 1, gemm::kMx4, AM>;
+  return f32 ? gemm::gemm_tn_kernel<128, float, 1, gemm::kMx4, AM> : gemm::gemm_tn_kernel<128, __nv_bfloat16, 1, gemm::kMx4, AM>;
+}
+
 KernelFn select_kernel(int bn, int dtype_c, int cta_group, int mx, int am) {
   const bool f32 = dtype_c == B200_F32 || dtype_c == B200_I32;  // 32-bit outputs share the store path
+  if (mx == gemm::kMx4 && am == 32) return select_kernel_mx4_skinny<32>(bn, f32);
+  if (mx == gemm::kMx4 && am == 64) return select_kernel_mx4_skinny<64>(bn, f32);
+  if (mx == gemm::kMx4 && bn == 64) return select_kernel_mx4_skinny<gemm::kBM>(bn, f32);
   if (am == 32) return select_kernel_short_a<32>(bn, f32);
   if (am == 64) return select_kernel_short_a<64>(bn, f32);
+  if (mx == gemm::kMx4 && bn == 192) return f32 ? gemm::gemm_tn_kernel<192, float, 2, gemm::kMx4> : gemm::gemm_tn_kernel<192, __nv_bfloat16, 2, gemm::kMx4>;
   if (mx == gemm::kMx4) return select_kernel_mx<gemm::kMx4>(bn, f32, cta_group);
   if (mx == gemm::kMx8) return select_kernel_mx<gemm::kMx8>(bn, f32, cta_group);
   return cta_group == 2 ? select_kernel_cg<2>(bn, f32) : select_kernel_cg<1>(bn, f32);
@@ -345,10 +356,11 @@ void plan_tail_split(b200_gemm_plan* plan) {
   // 3-5 us (export, fence, flag, read back), a K block of a full-width tile about 0.36 us, so a
   // split that saves fewer than ~12 K blocks per unit makes the launch longer (512^3: 8 K blocks,
   // 9.3 -> 6 us per launch without the split).
-  constexpr int kMinKbPerPart = 12;
+  // (4-bit: twice that -- an SM alone streams a short tile faster than two exchange it.)
+  const int min_kb_per_part = plan->mx == gemm::kMx4 ? 24 : 12;
   int parts = 0;
   for (int cand = 8; cand >= 2; cand /= 2) {
-    if (cand > units / tail || plan->bn / cand < 32 || plan->num_kb / cand < kMinKbPerPart) continue;
+    if (cand > units / tail || plan->bn / cand < 32 || plan->bn % (32 * cand) != 0 || plan->num_kb / cand < min_kb_per_part) continue;
     const int per = (plan->num_kb + cand - 1) / cand;
     if ((plan->num_kb + per - 1) / per != cand) continue;
     parts = cand;
@@ -363,9 +375,9 @@ void plan_tail_split(b200_gemm_plan* plan) {
   // One round, one part per CTA (skinny problems: a few column tiles, a long K): the parts of a
   // tile form a cluster and exchange through its shared memory.  The parking area (a 128 x BN
   // fp32 tile) must fit in the stage ring.  reserved[1] bit 2 keeps the exchange in the workspace.
-  if (plan->cg == 1 && plan->mx == gemm::kMxNone && plan->cluster_exchange_ok && (plan->desc.reserved[1] & 4) == 0 && tail == tiles &&
+  if (plan->cg == 1 && plan->mx != gemm::kMx8 && plan->cluster_exchange_ok && (plan->desc.reserved[1] & 4) == 0 && tail == tiles &&
       tiles * parts <= units &&
-      static_cast<int64_t>(plan->stages) * gemm::stage_bytes(plan->bn, 1, gemm::kMxNone, plan->am) >= static_cast<int64_t>(gemm::kBM) * plan->bn * 4) {
+      static_cast<int64_t>(plan->stages) * gemm::stage_bytes(plan->bn, 1, plan->mx, plan->am) >= static_cast<int64_t>(gemm::kBM) * plan->bn * 4) {
     plan->cluster_exchange = true;
     return;  // no flags, no partial tiles in global memory
   }
@@ -657,7 +669,9 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
   if (mx != gemm::kMxNone) {
     B200_REQUIRE(d.K % 32 == 0, "gemm_plan_create: block-scaled inputs need K %% 32 == 0 (one scale per 32 elements), got K=%lld", (long long)d.K);
     B200_REQUIRE(d.b_layout == B200_B_ROW_MAJOR_NK, "gemm_plan_create: block-scaled inputs take row-major B");
-    B200_REQUIRE(d.tile_n == 0 || d.tile_n == 128 || d.tile_n == 256, "gemm_plan_create: block-scaled inputs use tile_n=128 or 256 (got %d)", d.tile_n);
+    B200_REQUIRE(d.tile_n == 0 || d.tile_n == 128 || d.tile_n == 256 || (mx == gemm::kMx4 && d.tile_n == 192 && d.cta_group != 1 && d.tile_m != gemm::kBM) ||
+                     (mx == gemm::kMx4 && d.tile_n == 64 && d.cta_group != 2 && d.tile_m != 2 * gemm::kBM),
+                 "gemm_plan_create: block-scaled inputs use tile_n=128 or 256, with fp4 also 64 (one CTA) and 192 (a CTA pair); got %d", d.tile_n);
     B200_REQUIRE(mx != gemm::kMx4 || d.split_k <= 1, "gemm_plan_create: 4-bit inputs do not split K through a workspace (split_k=%d)", d.split_k);
   }
   B200_REQUIRE(d.dtype_c == B200_F32 || d.dtype_c == B200_BF16 || d.dtype_c == B200_I32,
@@ -680,7 +694,7 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
   }
   B200_REQUIRE(d.tile_m == 0 || d.tile_m == gemm::kBM || d.tile_m == 2 * gemm::kBM,
                "gemm_plan_create: tile_m=%d unsupported (128, or 256 for a CTA pair)", d.tile_m);
-  B200_REQUIRE(d.tile_n == 0 || d.tile_n == 32 || d.tile_n == 64 || d.tile_n == 128 || d.tile_n == 256,
+  B200_REQUIRE(d.tile_n == 0 || d.tile_n == 32 || d.tile_n == 64 || d.tile_n == 128 || d.tile_n == 256 || (d.tile_n == 192 && mx == gemm::kMx4),
                "gemm_plan_create: tile_n=%d unsupported (32, 64, 128, 256)", d.tile_n);
   const int kb_elems = mx == gemm::kMx4 ? gemm::kMx4StageElems : gemm::kRowBytes / eb;
   B200_REQUIRE(d.tile_k == 0 || d.tile_k == kb_elems, "gemm_plan_create: tile_k=%d unsupported (%d for this dtype)", d.tile_k, kb_elems);
@@ -715,6 +729,40 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
   // stages, one epilogue -- which more and smaller CTAs shorten (one CTA per 128 x 32 tile:
   // 6.7 us per launch against 7.9 us for pairs on 256 x 64 tiles).
   const bool short_k = k_blocks <= 16;
+  // 4-bit operands: the tile (and with it one or two CTAs) whose rounds cost least.  A stage costs what the L2
+  // sends its SM, about 100 GB/s: 26.6 KB for a pair's 256 x 128, 31.7 for 256 x 192, 35.8 for 256 x 256 and
+  // 34.8 for one CTA's 128 x 128, which measures a little faster than that; a tile costs 1.2 us on top, but
+  // 5 us with 256 columns, whose single accumulator keeps the MMAs waiting.  Measured (us; 128 / 192 / 256
+  // columns on pairs, 128 on one CTA): 8192^3 232 / 188 / 224, 279; 4096^3 40.6 / 33.7 / 42.0, 42.4;
+  // 512 x 8192 x 8192 21.7 / 23.6 / 18.3, 22.5; 256 x 8192 x 8192 14.2 / 15.5 / 17.0, 13.6.
+  //
+  // Up to 128 rows the product streams B from DRAM: one CTA per tile, and the width whose rounds move the
+  // fewest columns per SM (16 x 8192 x 8192: 9.6 us with 128 tiles of 64 columns, 12.5 with 64 of 128, each
+  // cut in two along K).
+  int mx4_bn = 0, mx4_cg = 0;
+  if (mx == gemm::kMx4 && d.tile_n == 0 && d.M <= gemm::kBM && cg != 2) {
+    cg = 1;
+    mx4_bn = ceil_div(ceil_div(d.N, 64), kDefaultSms) * 64 < ceil_div(ceil_div(d.N, 128), kDefaultSms) * 128 ? 64 : 128;
+  } else if (mx == gemm::kMx4 && d.tile_n == 0) {
+    static const struct {
+      int cg, bn;
+      double stage_us, tile_us;
+    } kTiles[] = {{1, 128, 0.31, 1.2}, {2, 128, 0.266, 1.2}, {2, 192, 0.317, 1.2}, {2, 256, 0.358, 5.0}};
+    double best = 0.0;
+    for (const auto& t : kTiles) {
+      if ((cg != 0 && t.cg != cg) || (cg == 0 && t.cg == 2 && d.M < 2 * gemm::kBM)) continue;
+      const int64_t tiles = static_cast<int64_t>(ceil_div(d.M, gemm::kBM * t.cg)) * ceil_div(d.N, t.bn), units = kDefaultSms / t.cg;
+      const double us = static_cast<double>((tiles + units - 1) / units) * (k_blocks * t.stage_us + t.tile_us);
+      if (mx4_bn == 0 || us < best - 1e-9) {
+        mx4_bn = t.bn;
+        mx4_cg = t.cg;
+        best = us;
+      }
+    }
+    cg = mx4_cg;
+  }
+  if (cg == 0 && d.tile_n == 192) cg = 2;
+  if (cg == 0 && mx == gemm::kMx4 && d.tile_n == 64) cg = 1;
   if (cg == 0) {
     cg = (d.b_layout == B200_B_ROW_MAJOR_NK && d.M >= 2 * gemm::kBM && d.tile_n != 32) ? 2 : 1;
     if (cg == 2 && short_k && mx == gemm::kMxNone && d.tile_n == 0 &&
@@ -735,7 +783,7 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
 
   // Tile width: the widest tile whose tile count still fills the machine; wide tiles halve the
   // shared-memory traffic per flop, narrow ones keep more SMs busy on small problems.
-  int bn = d.tile_n;
+  int bn = mx4_bn != 0 ? mx4_bn : d.tile_n;
   if (bn == 0 && mx != gemm::kMxNone) {
     // 256 columns unless that leaves SMs without a tile: a 128-column tile is bound by shared-memory reads.
     bn = (static_cast<int64_t>(plan->m_blocks) * ceil_div(d.N, 256) >= kDefaultSms / cg) ? 256 : 128;
@@ -801,7 +849,7 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
   // ring holds more of B, the operand that such a problem streams from HBM.  tile_m = 128
   // asks for full A stages.
   int am = gemm::kBM;
-  if (cg == 1 && mx == gemm::kMxNone && d.tile_m == 0 && d.M <= 64 && (bn == 64 || bn == 128)) am = d.M <= 32 ? 32 : 64;
+  if (cg == 1 && mx != gemm::kMx8 && d.tile_m == 0 && d.M <= 64 && (bn == 64 || bn == 128)) am = d.M <= 32 ? 32 : 64;
   plan->am = am;
   // Full-A stages never profit from more than 8 slots.  Short-A stages belong to problems that
   // stream B from HBM, and a stream of 16 KB copies is fastest with about 100 KB per SM on request
@@ -810,7 +858,7 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
   const int b_stage_bytes = bn / cg * gemm::kRowBytes;
   const int short_a_cap = std::max(4, std::min(gemm::kMaxStages, (112 * 1024 + b_stage_bytes - 1) / b_stage_bytes));
   const int stage_cap = am < gemm::kBM ? short_a_cap : 8;
-  const int max_stages = (kMaxSmemOptin - gemm::kBarrierBytes - 1024 - gemm::a_overrun_bytes(bn, cg, mx, am)) / gemm::stage_bytes(bn, cg, mx, am);
+  const int max_stages = (kMaxSmemOptin - gemm::kBarrierBytes - 1024 - gemm::c_store_bytes(mx, am) - gemm::a_overrun_bytes(bn, cg, mx, am)) / gemm::stage_bytes(bn, cg, mx, am);
   int stages = d.stages > 0 ? d.stages : (max_stages < stage_cap ? max_stages : stage_cap);
   if (stages > max_stages) {
     delete plan;

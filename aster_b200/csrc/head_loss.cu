@@ -322,7 +322,9 @@ struct Tiling {
 
 int ring(Tiling* t) {
   const int room = kMaxSmem - head::kBarrierBytes - 1024 - head::overrun_bytes(t->bn, t->cg, t->am);
-  t->stages = std::min(8, room / head::stage_bytes(t->bn, t->cg, t->am));
+  // With few rows the product streams w from DRAM, which is fastest with about 112 KB of it on request per SM.
+  const int cap = t->am < 128 ? std::max(4, 112 * 1024 / (t->bn * head::kRowBytes)) : 8;
+  t->stages = std::min(cap, room / head::stage_bytes(t->bn, t->cg, t->am));
   t->smem = head::smem_bytes(t->bn, t->stages, t->cg, t->am);
   // One CTA per SM: each takes all of TMEM.
   if (t->smem <= kMaxSmem / 2) t->smem = kMaxSmem / 2 + 1024;

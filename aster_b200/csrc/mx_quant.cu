@@ -12,20 +12,28 @@
 // row r of a block at byte (r % 32) * 16 + (r / 32) * 4; see pack_mx_scales_kernel), so that no
 // second pass over them is needed.
 //
-// Both kernels are bound by DRAM: a lane moves 8 values (16 or 32 bytes, one vector access) and 4
-// lanes share a block, so a warp's accesses are contiguous and the block maximum is two shuffles.
+// Both kernels are bound by DRAM.  A lane moves 8 values (16 or 32 bytes, one vector access) and 4 lanes
+// share a block, so a warp's accesses are contiguous and the block maximum is two shuffles.  A CTA covers
+// 128 rows x 256 of K, which are exactly two scale blocks: they pass through shared memory and leave (or
+// arrive) as whole lines, where single bytes or words would be partial sectors of 32 rows.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp4.h>
 
 #include "common.h"
+#include "ptx_sm100.cuh"
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPerLane = 8;               // values per lane and step
-constexpr int kChunk = 32 * kPerLane;     // values per warp and step: 8 blocks of 32, 2 scale words
-constexpr int kSteps = 4;                 // chunks per warp, loads of all of them in flight together
+constexpr int kWarps = kThreads / 32;
+constexpr int kPerLane = 8;               // values per lane and row
+constexpr int kTileK = 32 * kPerLane;     // of K per CTA: 8 blocks of 32 per row
+constexpr int kTileRows = 128;
+// Rows per warp whose loads are in flight together: 8 vectors of 16 bytes per lane, either type.
+template <typename T>
+constexpr int kAhead = 128 / static_cast<int>(sizeof(T) * kPerLane);
+constexpr int kCodesAhead = 8;  // likewise when reading codes
 constexpr int kScaleBlockBytes = 512;
 
 // 8 consecutive values as raw 32-bit words.
@@ -82,77 +90,100 @@ __device__ __forceinline__ uint32_t e2m1_pair(float lo, float hi) {
   return static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(make_float2(lo, hi), __NV_E2M1, cudaRoundNearest));
 }
 
-// Position of the 4-byte scale word of (row, 128-element K group `kg`) in the packed scales.
-__device__ __forceinline__ size_t scale_word(int64_t row, int64_t kg, int64_t k_groups) {
-  const int r = static_cast<int>(row & 127);
-  return static_cast<size_t>((row >> 7) * k_groups + kg) * kScaleBlockBytes + static_cast<size_t>((r & 31) * 16 + (r >> 5) * 4);
+// Byte of (row r of 128, block kb of 8) in a CTA's two scale blocks.
+__device__ __forceinline__ int scale_at(int r, int kb) { return (kb >> 2) * kScaleBlockBytes + (r & 31) * 16 + (r >> 5) * 4 + (kb & 3); }
+
+// The CTA's tile: blockIdx.x counts 256-column tiles fastest.
+struct Tile {
+  int64_t row0, k0;
+  int rows;       // rows that exist
+  int groups;     // scale blocks (128 of K) that exist: 1 or 2
+  size_t scales;  // first byte of the first one
+};
+__device__ __forceinline__ Tile tile_of(int64_t rows, int64_t K, unsigned tiles_k) {
+  Tile t;
+  const unsigned rb = blockIdx.x / tiles_k;
+  const unsigned kt = blockIdx.x - rb * tiles_k;
+  t.row0 = static_cast<int64_t>(rb) * kTileRows;
+  t.k0 = static_cast<int64_t>(kt) * kTileK;
+  t.rows = static_cast<int>(rows - t.row0 < kTileRows ? rows - t.row0 : kTileRows);
+  const int64_t k_groups = (K + 127) / 128;
+  t.groups = k_groups - 2 * static_cast<int64_t>(kt) >= 2 ? 2 : 1;
+  t.scales = (static_cast<size_t>(rb) * k_groups + 2 * static_cast<size_t>(kt)) * kScaleBlockBytes;
+  return t;
 }
 
-// `rows_padded`: rows rounded up to 128; the rows behind the last only get scale bytes of 127, so
-// that every byte of the packed scales is defined.
+// Rows behind the last and blocks behind K get scale bytes of 127, so that every byte of the packed
+// scales is defined.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kThreads) quantize_mx4_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ scales,
-                                                                int64_t rows, int64_t rows_padded, int64_t K, int64_t row_stride,
-                                                                int64_t chunks) {
-  const int lane = threadIdx.x & 31;
-  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  const int64_t k_groups = (K + 127) / 128;
-  const int64_t total = rows_padded * chunks;
-  Raw<T> raw[kSteps];
+                                                                int64_t rows, int64_t K, int64_t row_stride, unsigned tiles_k) {
+  __shared__ __align__(16) uint8_t s_scale[2 * kScaleBlockBytes];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Tile t = tile_of(rows, K, tiles_k);
+  reinterpret_cast<uint32_t*>(s_scale)[threadIdx.x] = 0x7F7F7F7Fu;  // 256 words
+  __syncthreads();
+  const int64_t k = t.k0 + lane * kPerLane;
+  const bool k_ok = k < K;
+  const T* const src = x + t.row0 * row_stride + k;
+  uint8_t* const dst = q + (t.row0 * K + k) / 2;
+#pragma unroll 1
+  for (int r0 = warp; r0 < t.rows; r0 += kWarps * kAhead<T>) {
+    Raw<T> raw[kAhead<T>];
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const int64_t item = warp * kSteps + s;
-    const int64_t row = item / chunks;
-    const int64_t k = (item - row * chunks) * kChunk + lane * kPerLane;
-    if (item < total && row < rows && k < K) {
-      raw[s] = load8<T, kVec>(x + row * row_stride + k);
-    } else {
+    for (int a = 0; a < kAhead<T>; ++a) {
+      const int r = r0 + a * kWarps;
+      if (r < t.rows && k_ok) {
+        raw[a] = load8<T, kVec>(src + r * row_stride);
+      } else {
 #pragma unroll
-      for (int j = 0; j < static_cast<int>(sizeof(raw[s].w) / 4); ++j) raw[s].w[j] = 0u;
+        for (int j = 0; j < static_cast<int>(sizeof(raw[a].w) / 4); ++j) raw[a].w[j] = 0u;
+      }
     }
-  }
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const int64_t item = warp * kSteps + s;
-    if (item >= total) break;  // warp-uniform
-    const int64_t row = item / chunks;
-    const int64_t chunk = item - row * chunks;
-    const int64_t k = chunk * kChunk + lane * kPerLane;
-    float v[kPerLane];
-    uint32_t amax = 0u;  // magnitudes compare as integers; infinities and NaN come out largest
+    for (int a = 0; a < kAhead<T>; ++a) {
+      const int r = r0 + a * kWarps;
+      float v[kPerLane];
+      uint32_t amax = 0u;  // magnitudes compare as integers; infinities and NaN come out largest
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      v[i] = value<T>(raw[s], i);
-      amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    }
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const uint32_t field = amax >> 23;  // biased exponent of the maximum; 0 below 2^-126
-    uint32_t byte = field > 2u ? field - 2u : 0u;
-    if (amax == 0u) byte = 127u;
-    const bool bad = field == 255u;
-    if (bad) byte = 255u;
-    const float inv = bad ? 0.0f : __uint_as_float((254u - byte) << 23);
-    uint32_t codes = 0u;
-    if (!bad) {
+      for (int i = 0; i < kPerLane; ++i) {
+        v[i] = value<T>(raw[a], i);
+        amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+      }
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const uint32_t field = amax >> 23;  // biased exponent of the maximum; 0 below 2^-126
+      uint32_t byte = field > 2u ? field - 2u : 0u;
+      if (amax == 0u) byte = 127u;
+      const bool bad = field == 255u;
+      if (bad) byte = 255u;
+      const float inv = __uint_as_float((254u - (bad ? 127u : byte)) << 23);
+      uint32_t codes = 0u;
 #pragma unroll
       for (int i = 0; i < kPerLane / 2; ++i) codes |= e2m1_pair(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
+      if (bad) codes = 0u;
+      if (r < t.rows && k_ok) {
+        *reinterpret_cast<uint32_t*>(dst + r * (K / 2)) = codes;
+        if ((lane & 3) == 0) s_scale[scale_at(r, lane >> 2)] = static_cast<uint8_t>(byte);
+      }
     }
-    if (row < rows && k < K) *reinterpret_cast<uint32_t*>(q + (row * K + k) / 2) = codes;
-    // Four blocks of 32 share a scale word: lanes 0 and 16 collect theirs.
-    uint32_t word = byte << (8 * ((lane >> 2) & 3));
-    word |= __shfl_xor_sync(0xffffffffu, word, 4);
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
-    const int64_t kg = chunk * 2 + (lane >> 4);
-    if ((lane & 15) == 0 && kg < k_groups) *reinterpret_cast<uint32_t*>(scales + scale_word(row, kg, k_groups)) = word;
+  }
+  __syncthreads();
+  if (threadIdx.x < t.groups * (kScaleBlockBytes / 16)) {
+    reinterpret_cast<uint4*>(scales + t.scales)[threadIdx.x] = reinterpret_cast<const uint4*>(s_scale)[threadIdx.x];
   }
 }
 
 // Rounding into the output type; for bf16 and fp32 it never rounds (two significant bits, and the
 // smallest value, 2^-128, is a bf16 subnormal).
 __device__ __forceinline__ void store8(float* p, const float (&v)[kPerLane]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  if ((reinterpret_cast<uintptr_t>(p) & 31u) != 0) {  // a caller's buffer may be aligned to 16 bytes only
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    return;
+  }
+  sm100::st_global_v8(p, __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]), __float_as_uint(v[4]),
+                      __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
 }
 __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[kPerLane]) {
   uint32_t w[4];
@@ -175,40 +206,43 @@ __device__ __forceinline__ void store8(__half* p, const float (&v)[kPerLane]) {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) dequantize_mx4_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales, T* __restrict__ out,
-                                                                  int64_t rows, int64_t K, int64_t chunks) {
-  const int lane = threadIdx.x & 31;
-  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  const int64_t k_groups = (K + 127) / 128;
-  const int64_t total = rows * chunks;
-  uint32_t codes[kSteps], byte[kSteps];
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const int64_t item = warp * kSteps + s;
-    const int64_t row = item / chunks;
-    const int64_t k = (item - row * chunks) * kChunk + lane * kPerLane;
-    codes[s] = byte[s] = 0u;
-    if (item < total && k < K) {
-      codes[s] = __ldcs(reinterpret_cast<const uint32_t*>(q + (row * K + k) / 2));
-      byte[s] = __ldg(scales + scale_word(row, k >> 7, k_groups) + ((k >> 5) & 3));
-    }
+                                                                  int64_t rows, int64_t K, unsigned tiles_k) {
+  __shared__ __align__(16) uint8_t s_scale[2 * kScaleBlockBytes];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Tile t = tile_of(rows, K, tiles_k);
+  const int64_t k = t.k0 + lane * kPerLane;
+  const bool k_ok = k < K;
+  const uint8_t* const src = q + (t.row0 * K + k) / 2;
+  T* const dst = out + t.row0 * K + k;
+  if (threadIdx.x < t.groups * (kScaleBlockBytes / 16)) {
+    reinterpret_cast<uint4*>(s_scale)[threadIdx.x] = __ldg(reinterpret_cast<const uint4*>(scales + t.scales) + threadIdx.x);
   }
+  __syncthreads();
+#pragma unroll 1
+  for (int r0 = warp; r0 < t.rows; r0 += kWarps * kCodesAhead) {
+    uint32_t codes[kCodesAhead];
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const int64_t item = warp * kSteps + s;
-    const int64_t row = item / chunks;
-    const int64_t k = (item - row * chunks) * kChunk + lane * kPerLane;
-    if (item >= total || k >= K) continue;
-    // 2^(byte - 127): below 2^-126 a subnormal, 255 is NaN
-    const float scale = byte[s] == 255u ? __uint_as_float(0x7FC00000u) : (byte[s] == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte[s] << 23));
-    float v[kPerLane];
-#pragma unroll
-    for (int i = 0; i < kPerLane / 2; ++i) {
-      const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>((codes[s] >> (8 * i)) & 0xFFu), __NV_E2M1);
-      const float2 f = __half22float2(__half2(h));
-      v[2 * i] = f.x * scale;
-      v[2 * i + 1] = f.y * scale;
+    for (int a = 0; a < kCodesAhead; ++a) {
+      const int r = r0 + a * kWarps;
+      codes[a] = r < t.rows && k_ok ? __ldcs(reinterpret_cast<const uint32_t*>(src + r * (K / 2))) : 0u;
     }
-    store8(out + row * K + k, v);
+#pragma unroll
+    for (int a = 0; a < kCodesAhead; ++a) {
+      const int r = r0 + a * kWarps;
+      if (r >= t.rows || !k_ok) continue;
+      const uint32_t byte = s_scale[scale_at(r, lane >> 2)];
+      // 2^(byte - 127): byte 0 is a subnormal, 255 is NaN
+      const float scale = byte == 255u ? __uint_as_float(0x7FC00000u) : (byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23));
+      float v[kPerLane];
+#pragma unroll
+      for (int i = 0; i < kPerLane / 2; ++i) {
+        const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>((codes[a] >> (8 * i)) & 0xFFu), __NV_E2M1);
+        const float2 f = __half22float2(__half2(h));
+        v[2 * i] = f.x * scale;
+        v[2 * i + 1] = f.y * scale;
+      }
+      store8(dst + r * K, v);
+    }
   }
 }
 
@@ -219,21 +253,18 @@ int check_shape(const char* who, int64_t rows, int64_t K, int dtype_q) {
   return B200_OK;
 }
 
-// One warp per kSteps chunks.
-int grid_for(const char* who, int64_t rows, int64_t chunks, unsigned* grid) {
-  const int64_t per_cta = static_cast<int64_t>(kSteps) * (kThreads / 32);
-  const int64_t ctas = (rows * chunks + per_cta - 1) / per_cta;
-  B200_REQUIRE(ctas < (1ll << 31), "%s: %lld x %lld chunks of 256 values are more than one launch covers", who, (long long)rows, (long long)chunks);
-  *grid = static_cast<unsigned>(ctas);
+int grid_for(const char* who, int64_t rows, int64_t K, unsigned* grid, unsigned* tiles_k) {
+  const int64_t tk = (K + kTileK - 1) / kTileK, tiles = (rows + kTileRows - 1) / kTileRows * tk;
+  B200_REQUIRE(tiles < (1ll << 31), "%s: %lld x %lld values are more than one launch covers", who, (long long)rows, (long long)K);
+  *grid = static_cast<unsigned>(tiles);
+  *tiles_k = static_cast<unsigned>(tk);
   return B200_OK;
 }
 
 template <typename T>
 int launch_quantize(const void* x, void* q, void* scales, int64_t rows, int64_t K, int64_t row_stride, cudaStream_t stream) {
-  const int64_t chunks = (K + kChunk - 1) / kChunk;
-  const int64_t padded = (rows + 127) / 128 * 128;
-  unsigned grid = 0;
-  const int rc = grid_for("quantize_mx", padded, chunks, &grid);
+  unsigned grid = 0, tiles_k = 0;
+  const int rc = grid_for("quantize_mx", rows, K, &grid, &tiles_k);
   if (rc != B200_OK) return rc;
   // Vector loads need every row to start on a 16-byte boundary (a lane's 8 values then do, too).
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && (row_stride * static_cast<int64_t>(sizeof(T))) % 16 == 0;
@@ -241,9 +272,9 @@ int launch_quantize(const void* x, void* q, void* scales, int64_t rows, int64_t 
   uint8_t* qb = static_cast<uint8_t*>(q);
   uint8_t* sb = static_cast<uint8_t*>(scales);
   if (vec) {
-    quantize_mx4_kernel<T, true><<<grid, kThreads, 0, stream>>>(xt, qb, sb, rows, padded, K, row_stride, chunks);
+    quantize_mx4_kernel<T, true><<<grid, kThreads, 0, stream>>>(xt, qb, sb, rows, K, row_stride, tiles_k);
   } else {
-    quantize_mx4_kernel<T, false><<<grid, kThreads, 0, stream>>>(xt, qb, sb, rows, padded, K, row_stride, chunks);
+    quantize_mx4_kernel<T, false><<<grid, kThreads, 0, stream>>>(xt, qb, sb, rows, K, row_stride, tiles_k);
   }
   b200::count_launch();
   B200_CUDA_OK(cudaGetLastError());
@@ -252,11 +283,10 @@ int launch_quantize(const void* x, void* q, void* scales, int64_t rows, int64_t 
 
 template <typename T>
 int launch_dequantize(const void* q, const void* scales, void* out, int64_t rows, int64_t K, cudaStream_t stream) {
-  const int64_t chunks = (K + kChunk - 1) / kChunk;
-  unsigned grid = 0;
-  const int rc = grid_for("dequantize_mx", rows, chunks, &grid);
+  unsigned grid = 0, tiles_k = 0;
+  const int rc = grid_for("dequantize_mx", rows, K, &grid, &tiles_k);
   if (rc != B200_OK) return rc;
-  dequantize_mx4_kernel<T><<<grid, kThreads, 0, stream>>>(static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scales), static_cast<T*>(out), rows, K, chunks);
+  dequantize_mx4_kernel<T><<<grid, kThreads, 0, stream>>>(static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scales), static_cast<T*>(out), rows, K, tiles_k);
   b200::count_launch();
   B200_CUDA_OK(cudaGetLastError());
   return B200_OK;

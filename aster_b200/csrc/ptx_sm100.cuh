@@ -162,6 +162,15 @@ __device__ __forceinline__ void bulk_load_1d(uint32_t smem_dst, const void* gsrc
                : "memory");
 }
 
+__device__ __forceinline__ void st_shared_u4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_u4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
 // ---------------------------------------------------------------------------------------------
 // tcgen05: tensor memory and MMA
 // ---------------------------------------------------------------------------------------------
@@ -414,8 +423,8 @@ __host__ __device__ constexpr uint32_t make_idesc_mx4(uint32_t umma_m, uint32_t 
       B200_MX4_CP(GROUP, 1, 4) B200_MX4_CP(GROUP, 2, 8) B200_MX4_CP(GROUP, 3, 16)               \
       B200_MX4_CP_IF(GROUP, 4, 12) B200_MX4_CP_IF(GROUP, 5, 20)                                 \
       "add.u32 ta1, %6, 4;\n"                                                                   \
-      "add.u32 tb0, %6, 8;\n"                                                                   \
-      "add.u32 tb1, %6, 16;\n"                                                                  \
+      "add.u32 tb0, %11, 8;\n"                                                                  \
+      "add.u32 tb1, %11, 16;\n"                                                                 \
       "setp.eq.b32 q, 0, 0;\n"                                                                  \
       "mov.b64 da, {%1, %3};\n"                                                                 \
       "mov.b64 db, {%2, %3};\n"                                                                 \
@@ -423,14 +432,15 @@ __host__ __device__ constexpr uint32_t make_idesc_mx4(uint32_t umma_m, uint32_t 
       B200_MX4_MMA(GROUP, 1, 1, "%6", "tb0") B200_MX4_MMA(GROUP, 2, 0, "ta1", "tb1")            \
       B200_MX4_MMA(GROUP, 3, 1, "ta1", "tb1") "}\n" ::"r"(tmem_d),                               \
       "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate_first), "r"(sf_tmem), "r"(sf_lo), "r"(sf_hi), "r"(NB), \
-      "r"(mmas)                                                                                 \
+      "r"(mmas), "r"(sf_tmem + sfb_shift)                                                       \
       : "memory")
 
 // One block-scaled 4-bit stage: the scale blocks (A half 0, A half 1, then the two halves of each
 // 128 rows of B, 512 bytes apart) go to TMEM, then the first `mmas` (1..4) MMAs of the stage.
+// `sfb_shift`: scale columns of B in front of the tile's first one (0, or 2 when it starts at row 64 of 128).
 template <int CTA_GROUP, int NB>
 __device__ __forceinline__ void umma_mx4_stage(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc,
-                                               uint32_t accumulate_first, uint32_t sf_tmem, uint32_t sf_lo, uint32_t mmas) {
+                                               uint32_t accumulate_first, uint32_t sf_tmem, uint32_t sf_lo, uint32_t mmas, uint32_t sfb_shift) {
   static_assert(NB == 1 || NB == 2, "one or two 128-row groups of B");
   constexpr uint32_t sf_hi = smem_desc_hi_scales();
   if constexpr (CTA_GROUP == 1) {

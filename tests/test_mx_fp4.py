@@ -105,6 +105,9 @@ class TestOnHost:
             GemmPlan(128, 128, 2048, "mxe2m1", "f32", split_k=2)
         with pytest.raises(nat.B200Error, match="row-major B"):
             GemmPlan(128, 128, 2048, "mxe2m1", "f32", b_layout="packed")
+        for bad in (dict(tile_n=64, cta_group=2), dict(tile_n=192, cta_group=1), dict(tile_n=32)):
+            with pytest.raises(nat.B200Error, match="tile_n"):
+                GemmPlan(512, 512, 2048, "mxe2m1", "f32", **bad)
         with pytest.raises(nat.B200Error, match="tile_k"):
             GemmPlan(128, 128, 2048, "mxe2m1", "f32", tile_k=128)
         assert GemmPlan(512, 512, 2048, "mxe2m1", "bf16").resources().tile_k == 256
@@ -212,12 +215,12 @@ class TestProductOnGpu:
         sb = rng.integers(124, 131, (N, K // 32)).astype(np.uint8)
         ones = dtypes.pack_e2m1(dtypes.f32_to_e2m1_codes(np.ones((max(M, N), K), np.float32)))
         want = 32.0 * (np.exp2(sa.astype(np.float64) - 127) @ np.exp2(sb.astype(np.float64) - 127).T)
-        for kw in ({}, {"tile_n": 128}, {"cta_group": 1}, {"cta_group": 1, "tile_n": 256}):
+        for kw in ({}, {"tile_n": 128}, {"cta_group": 1}, {"cta_group": 1, "tile_n": 256}, {"tile_n": 192}, {"tile_n": 192, "max_ctas": 2}):
             got = gemm(ones[:M], ones[:N], dtype_ab="mxe2m1", dtype_c="f32", block_scales_a=sa, block_scales_b=sb, **kw)
             assert np.array_equal(got, want.astype(np.float32)), kw
 
     @pytest.mark.parametrize("plan", [{}, {"cta_group": 1, "tile_n": 128}, {"cta_group": 1, "tile_n": 256}, {"cta_group": 2, "tile_n": 128},
-                                      {"cta_group": 2, "tile_n": 256}, {"stages": 2}, {"max_ctas": 4}])
+                                      {"cta_group": 2, "tile_n": 256}, {"tile_n": 192}, {"tile_n": 64}, {"tile_n": 64, "tile_m": 128}, {"stages": 2}, {"max_ctas": 4}])
     @pytest.mark.parametrize("shape", SHAPES)
     def test_exact_sums(self, gpu, shape, plan):
         M, N, K = shape
@@ -230,8 +233,8 @@ class TestProductOnGpu:
         assert np.array_equal(got, dtypes.bf16_round(want.astype(np.float32)))
 
     @pytest.mark.parametrize("extra", [{}, {"max_ctas": 4, "tail_split": True}, {"cta_group": 1, "tile_n": 128, "max_ctas": 3, "tail_split": True},
-                                       {"cta_group": 2, "tile_n": 256, "max_ctas": 2, "tail_split": True}, {"static_b": True},
-                                       {"static_b": True, "cta_group": 1, "stages": 2}, {"split_k": -1}])
+                                       {"cta_group": 2, "tile_n": 256, "max_ctas": 2, "tail_split": True}, {"tile_n": 192, "max_ctas": 6, "tail_split": True}, {"tile_n": 192, "max_ctas": 2}, {"static_b": True},
+                                       {"static_b": True, "cta_group": 1, "stages": 2}, {"split_k": -1}, {"tile_n": 64, "max_ctas": 3}])
     def test_epilogue_and_schedules(self, gpu, extra):
         M, N, K = 384, 256, 6144 + 32
         rng = np.random.default_rng(9)
@@ -240,6 +243,17 @@ class TestProductOnGpu:
         want = np.maximum(product(a, b) + bias, 0).astype(np.float32)
         got = gemm(qa, qb, dtype_ab="mxe2m1", dtype_c="f32", block_scales_a=sa, block_scales_b=sb, bias=bias, relu=True, **extra)
         assert np.array_equal(got, want)
+
+    @pytest.mark.parametrize("M", [1, 17, 40, 100])
+    @pytest.mark.parametrize("N", [64, 200, 4096, 9500])
+    def test_few_rows(self, gpu, M, N):
+        """The forms that stream B: 64- and 128-column tiles, short A stages, and K cut between the CTAs of a cluster."""
+        for K, extra in ((2080, {}), (16384, {}), (16384, {"tile_n": 128}), (16384, {"tile_n": 64})):
+            rng = np.random.default_rng(M + N + K)
+            (qa, sa, a), (qb, sb, b) = exact_operand(M, K, rng, 127, 127), exact_operand(N, K, rng, 127, 127)
+            want = a @ b.T  # multiples of 1/4 below 36 * 16384 < 2^24 / 4
+            got = gemm(qa, qb, dtype_ab="mxe2m1", dtype_c="f32", block_scales_a=sa, block_scales_b=sb, **extra)
+            assert np.array_equal(got, want.astype(np.float32)), (K, extra)
 
     def test_nan_scales_stay_in_their_rows(self, gpu):
         """A NaN block in one row of A or B reaches that row or column of C only, wherever the data ends
