@@ -1014,12 +1014,15 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             __syncwarp();
             const int col = col0 + rd_chunk * (kCols / 8);
             OutT* dst = C + static_cast<size_t>(row0 + rd_row) * p.N + col;
+            uint4 t[8];  // all reads before the first store: their latencies overlap
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int r = 4 * i + rd_row;
-              const uint4 t = ld_shared_u4(buf + static_cast<uint32_t>(r) * 128u + ((static_cast<uint32_t>(rd_chunk) ^ static_cast<uint32_t>(r & 7)) << 4));
-              if (row0 + r < p.M && col < p.N) *reinterpret_cast<uint4*>(dst) = t;  // a 16-byte piece exists or does not
-              dst += static_cast<size_t>(4) * p.N;
+              t[i] = ld_shared_u4(buf + static_cast<uint32_t>(r) * 128u + ((static_cast<uint32_t>(rd_chunk) ^ static_cast<uint32_t>(r & 7)) << 4));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (row0 + 4 * i + rd_row < p.M && col < p.N) *reinterpret_cast<uint4*>(dst + static_cast<size_t>(4 * i) * p.N) = t[i];  // a 16-byte piece exists or does not
             }
           }
           lo = hi;  // nothing left for the loops below; a slab without rows is handed back there

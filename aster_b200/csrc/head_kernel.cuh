@@ -104,8 +104,11 @@ __host__ __device__ constexpr int overrun_bytes(int bn, int cg, int am) {
   return kBM * kRowBytes > stage_bytes(bn, cg, am) ? kBM * kRowBytes - stage_bytes(bn, cg, am) : 0;
 }
 constexpr int kBarrierBytes = 384;
+// 4 KB per epilogue warp in which 32 rows x 128 bytes of output are turned around (a lane per row writes them,
+// eight lanes per row read them), so that they leave as whole lines.
+constexpr int kTurnBytes = 32 * 128;
 __host__ __device__ constexpr int smem_bytes(int bn, int stages, int cg, int am) {
-  return stages * stage_bytes(bn, cg, am) + overrun_bytes(bn, cg, am) + kBarrierBytes + 1024;
+  return stages * stage_bytes(bn, cg, am) + gemm::kEpilogueWarps * kTurnBytes + overrun_bytes(bn, cg, am) + kBarrierBytes + 1024;
 }
 
 // 2^x for the softmax: the hardware's approximation (2 ulp) with results below 2^-126 flushed; the
@@ -222,27 +225,24 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 32 consecutive 16-bit outputs of a row.  `align`: bytes that every chunk of the row is aligned to
-// (32, 16, or less: element by element); `valid`: columns that exist.
-template <typename T>
-__device__ __forceinline__ void store32(T* dst, const float (&x)[32], int align, int valid) {
-  uint32_t w[16];
+// Turns the warp's 32 rows x 128 bytes around: lane l brings row l as 32 words and gets 16-byte pieces of
+// rows 4 i + l / 8, piece l % 8, for i = 0..7, handed to `use(i, piece)`.
+template <typename Use>
+__device__ __forceinline__ void turn_around(uint32_t buf, const uint32_t (&w)[32], Use use) {
+  const uint32_t lane = threadIdx.x & 31;
+  const uint32_t wr = buf + lane * 128u, wr_swz = (lane & 7u) << 4;
+  __syncwarp();  // the previous pieces have been read
 #pragma unroll
-  for (int j = 0; j < 16; ++j) w[j] = pack2<T>(x[2 * j], x[2 * j + 1]);
-  if (valid >= 32 && align >= 32) {
-    sm100::st_global_v8(dst, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
-    sm100::st_global_v8(dst + 16, w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15]);
-  } else if (valid >= 32 && align >= 16) {
-    uint4* d = reinterpret_cast<uint4*>(dst);
+  for (uint32_t j = 0; j < 8; ++j) sm100::st_shared_u4(wr + ((j << 4) ^ wr_swz), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  __syncwarp();
+  uint4 t[8];  // all reads before the first use: their latencies overlap
 #pragma unroll
-    for (int j = 0; j < 4; ++j) d[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-  } else {
-    unsigned short* d = reinterpret_cast<unsigned short*>(dst);
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      if (j < valid) d[j] = static_cast<unsigned short>((j & 1) ? (w[j >> 1] >> 16) : (w[j >> 1] & 0xFFFFu));
-    }
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t r = 4u * i + (lane >> 3);
+    t[i] = sm100::ld_shared_u4(buf + r * 128u + (((lane & 7u) ^ (r & 7u)) << 4));
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) use(i, t[i]);
 }
 
 // A row's labels during the walk over a tile's columns, in rising order.
@@ -322,7 +322,9 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
   const uint32_t b_rows = static_cast<uint32_t>(p.bn) / CG;
   const uint32_t b_bytes = b_rows * kRowBytes;
   const uint32_t st_bytes = a_bytes + b_bytes;
-  const uint32_t bar_base = smem_base + static_cast<uint32_t>(p.stages) * st_bytes + static_cast<uint32_t>(overrun_bytes(p.bn, CG, p.am));
+  // (what a short A stage's 128-row read touches behind the ring is the turn-around buffers, and what follows them)
+  [[maybe_unused]] const uint32_t turn_base = smem_base + static_cast<uint32_t>(p.stages) * st_bytes;
+  const uint32_t bar_base = turn_base + gemm::kEpilogueWarps * kTurnBytes + static_cast<uint32_t>(overrun_bytes(p.bn, CG, p.am));
   uint8_t* bar_ptr = smem_raw + (bar_base - smem_raw_u32);
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 128u + 8u * s; };
@@ -590,64 +592,85 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
         const float coef = row_ok ? __ldg(p.coef + row) : 0.0f;
         const float lse2 = row_ok ? __ldg(p.lse + row) * 1.4426950408889634f : 0.0f;
         const float shift = coef * p.base;
-        T16* const dst = static_cast<T16*>(p.g) + static_cast<size_t>(row_ok ? row : 0) * p.g_ld + tile_col;
+        const int piece_row = row - lane + (lane >> 3), piece_col = (lane & 7) * 8;  // of every 4 rows, of every 64 columns
+        T16* const dst = static_cast<T16*>(p.g) + static_cast<size_t>(piece_row) * p.g_ld + tile_col + piece_col;
 #pragma unroll 1
-        for (int c = 0; c < (slab_ok ? cols : 0); c += 32) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(taddr + static_cast<uint32_t>(c), v);
+        for (int c = 0; c < (slab_ok ? cols : 0); c += 64) {
+          uint32_t v[64];
+          tmem_ld_32x32b_x64(taddr + static_cast<uint32_t>(c), v);
           tmem_ld_wait();
-          float x[32];
+          uint32_t out[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) x[j] = fmaf(coef, ex2(fmaf(__uint_as_float(v[j]), p.scale2, -lse2)), -shift);
-          if (coef == 0.0f) {  // a row without a loss has no gradient, whatever its logits are
+          for (int h = 0; h < 2; ++h) {
+            float x[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) x[j] = 0.0f;
-          }
-          const int end = vcol + c + 32;
-          while (__any_sync(0xffffffffu, l.next < end)) {
-            if (l.next < end) {
-              const int at = l.next - (vcol + c);
-              const float d = coef * l.prob;
+            for (int j = 0; j < 32; ++j) x[j] = fmaf(coef, ex2(fmaf(__uint_as_float(v[32 * h + j]), p.scale2, -lse2)), -shift);
+            if (coef == 0.0f) {  // a row without a loss has no gradient, whatever its logits are
 #pragma unroll
-              for (int j = 0; j < 32; ++j) x[j] -= at == j ? d : 0.0f;
-              l.advance();
+              for (int j = 0; j < 32; ++j) x[j] = 0.0f;
             }
-            __syncwarp();
+            const int col = vcol + c + 32 * h;
+            const int end = c + 32 * h < cols ? col + 32 : 0;  // a tile may end after the first half
+            while (__any_sync(0xffffffffu, l.next < end)) {
+              if (l.next < end) {
+                const int at = l.next - col;
+                const float d = coef * l.prob;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] -= at == j ? d : 0.0f;
+                l.advance();
+              }
+              __syncwarp();
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) out[16 * h + j] = pack2<T16>(x[2 * j], x[2 * j + 1]);
           }
-          if (row_ok) store32<T16>(dst + c, x, 32, 32);  // rows of G are whole 64-column groups
-          __syncwarp();
+          // Rows of G are whole 64-column groups: what a piece writes behind the last column is never read.
+          const bool col_ok = c + piece_col < cols;
+          turn_around(turn_base + static_cast<uint32_t>(quarter) * kTurnBytes, out, [&](int i, const uint4& t) {
+            if (col_ok && piece_row + 4 * i < q.M) *reinterpret_cast<uint4*>(dst + static_cast<size_t>(4 * i) * p.g_ld + c) = t;
+          });
         }
       } else {
-        const bool out16 = q.out16 != nullptr;
-        T16* const dst = static_cast<T16*>(q.out16) + static_cast<size_t>(row_ok ? row : 0) * q.ld + tile_col;
-        float* const part = out16 ? nullptr : q.partial + (static_cast<size_t>(w.split) * q.M + (row_ok ? row : 0)) * q.N + tile_col;
-        const int align = (q.ld % 16 == 0 && (reinterpret_cast<uintptr_t>(q.out16) & 31u) == 0) ? 32 : 16;
+        const int piece_row = row - lane + (lane >> 3);
+        if (q.out16 != nullptr) {
+          const int piece_col = (lane & 7) * 8;
+          T16* const dst = static_cast<T16*>(q.out16) + static_cast<size_t>(piece_row) * q.ld + tile_col + piece_col;
 #pragma unroll 1
-        for (int c = 0; c < (slab_ok ? cols : 0); c += 32) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(taddr + static_cast<uint32_t>(c), v);
-          tmem_ld_wait();
-          float x[32];
+          for (int c = 0; c < (slab_ok ? cols : 0); c += 64) {
+            uint32_t v[64];
+            tmem_ld_32x32b_x64(taddr + static_cast<uint32_t>(c), v);
+            tmem_ld_wait();
+            uint32_t out[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(v[j]) * unscale;
-          const int valid = cols - c;
-          if (row_ok && out16) {
-            store32<T16>(dst + c, x, align, valid);
-          } else if (row_ok) {
+            for (int j = 0; j < 32; ++j) out[j] = pack2<T16>(__uint_as_float(v[2 * j]) * unscale, __uint_as_float(v[2 * j + 1]) * unscale);
+            const bool col_ok = c + piece_col < cols;  // the columns are a multiple of 8: a piece exists or does not
+            turn_around(turn_base + static_cast<uint32_t>(quarter) * kTurnBytes, out, [&](int i, const uint4& t) {
+              if (col_ok && piece_row + 4 * i < q.M) *reinterpret_cast<uint4*>(dst + static_cast<size_t>(4 * i) * q.ld + c) = t;
+            });
+          }
+        } else {
+          const int piece_col = (lane & 7) * 4;
+          float* const dst = q.partial + (static_cast<size_t>(w.split) * q.M + piece_row) * q.N + tile_col + piece_col;
+#pragma unroll 1
+          for (int c = 0; c < (slab_ok ? cols : 0); c += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(taddr + static_cast<uint32_t>(c), v);
+            tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              if (j < valid) {  // N is a multiple of 8
-                float4* d = reinterpret_cast<float4*>(part + c + j);
-                float4 t = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * unscale);
+            const bool col_ok = c + piece_col < cols;
+            turn_around(turn_base + static_cast<uint32_t>(quarter) * kTurnBytes, v, [&](int i, const uint4& t) {
+              if (col_ok && piece_row + 4 * i < q.M) {
+                float4* const d = reinterpret_cast<float4*>(dst + static_cast<size_t>(4 * i) * q.N + c);
+                float4 f = make_float4(__uint_as_float(t.x), __uint_as_float(t.y), __uint_as_float(t.z), __uint_as_float(t.w));
                 if (q.accumulate) {
                   const float4 o = *d;
-                  t = make_float4(t.x + o.x, t.y + o.y, t.z + o.z, t.w + o.w);
+                  f = make_float4(f.x + o.x, f.y + o.y, f.z + o.z, f.w + o.w);
                 }
-                *d = t;
+                *d = f;
               }
-            }
+            });
           }
-          __syncwarp();
         }
       }
       tc_fence_before_sync();

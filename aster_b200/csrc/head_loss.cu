@@ -321,7 +321,7 @@ struct Tiling {
 };
 
 int ring(Tiling* t) {
-  const int room = kMaxSmem - head::kBarrierBytes - 1024 - head::overrun_bytes(t->bn, t->cg, t->am);
+  const int room = kMaxSmem - head::kBarrierBytes - 1024 - gemm::kEpilogueWarps * head::kTurnBytes - head::overrun_bytes(t->bn, t->cg, t->am);
   // With few rows the product streams w from DRAM, which is fastest with about 112 KB of it on request per SM.
   const int cap = t->am < 128 ? std::max(4, 112 * 1024 / (t->bn * head::kRowBytes)) : 8;
   t->stages = std::min(cap, room / head::stage_bytes(t->bn, t->cg, t->am));
