@@ -44,6 +44,15 @@ enum Mode : int { kStats = 0, kGrad = 1, kProduct = 2 };
 // Codes of the status words, beside those of the GEMM kernel (status[1..2] = block, item).
 constexpr int kStatusWords = 16;
 
+// Division by a launch constant: floor(n / d) for 0 <= n, d < 2^31 as the high word of n 2 (floor(2^63 / d) + 1).
+// (The excess of the factor over 2^63 / d is at most 1, so the product is off by less than n / 2^63 < 1 / d.)
+struct FastDiv {
+  uint64_t m;
+  int d;
+  __host__ __device__ static FastDiv of(int d) { return {(1ull << 63) / static_cast<uint64_t>(d) + 1u, d}; }
+  __device__ __forceinline__ int div(int n) const { return static_cast<int>(__umul64hi(static_cast<uint64_t>(n) << 1, m)); }
+};
+
 struct Problem {
   int M, N;          // rows of A, rows of B (columns of the tile space)
   int num_kb;        // K blocks over the whole K
@@ -52,6 +61,10 @@ struct Problem {
   int m_blocks, n_blocks;
   int raster_group;
   int items;         // m_blocks * n_blocks * splits
+  FastDiv tiles;     // m_blocks * n_blocks
+  FastDiv span;      // raster_group * n_blocks
+  FastDiv group;     // raster_group
+  FastDiv last_group;  // m-blocks of the last raster group
   int a_mn, b_mn;    // operand lies with its rows along K
   int a_row0, b_row0;  // first row of A / B in their tensor maps
   int a_k0, b_k0;    // first K coordinate in their tensor maps
@@ -69,7 +82,7 @@ struct Params {
   int bn;            // tile width
   int am;            // rows of A per stage: 128, or 32 / 64 when M is no larger (one CTA, K-major)
   int stages;
-  int extra_rounds;  // see nth_item
+  int extra_rounds;  // see Walk
   uint32_t* status;
   unsigned wait_limit_ms;
   // labels: `top` entries per row in rising order of their ids (top = 1: the target itself)
@@ -166,27 +179,52 @@ __device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr, int mn) {
   return ((smem_addr >> 4) & 0x3FFFu) | ((mn ? static_cast<uint32_t>(kBoxBytes >> 4) : 1u) << 16);
 }
 
-// The i-th item of a unit (CTA or pair), or -1.  Items of problem 0 (the longer ones) are dealt
-// round-robin; the units that got one fewer then take `extra_rounds` items of problem 1 more, which is
-// how many of them take as long as one of problem 0, and the rest is dealt round-robin again.
-__device__ __forceinline__ int nth_item(const Params& p, int unit, int units, int i) {
-  const int items0 = p.prob[0].items;
-  const int total = items0 + (p.num_probs > 1 ? p.prob[1].items : 0);
-  const int rem = items0 % units;
-  const int mine0 = items0 / units + (unit < rem ? 1 : 0);
-  if (i < mine0) return unit + i * units;
-  i -= mine0;
-  const int extra = rem != 0 ? p.extra_rounds : 0;
-  if (rem != 0 && unit >= rem) {
-    if (i < extra) {
-      const int item = items0 + (unit - rem) + i * (units - rem);
-      return item < total ? item : -1;
-    }
-    i -= extra;
+// The items of a unit (CTA or pair), one after the other, -1 at the end.  Items of problem 0 (the longer ones)
+// are dealt round-robin; the units that got one fewer then take `extra_rounds` items of problem 1 more, which
+// is how many of them take as long as one of problem 0, and the rest is dealt round-robin again.
+struct Walk {
+  int at, step;       // next item of the current phase
+  int left;           // items left in it
+  int extra_at, extra_step, extra_left;
+  int rest_at, units, total;
+
+  __device__ __forceinline__ Walk(const Params& p, int unit, int n_units) {
+    const int items0 = p.prob[0].items;
+    const int rem = items0 % n_units;
+    units = n_units;
+    total = items0 + (p.num_probs > 1 ? p.prob[1].items : 0);
+    at = unit;
+    step = n_units;
+    left = items0 / n_units + (unit < rem ? 1 : 0);
+    const int extra = rem != 0 ? p.extra_rounds : 0;
+    extra_at = items0 + unit - rem;
+    extra_step = n_units - rem;
+    extra_left = rem != 0 && unit >= rem ? extra : 0;
+    rest_at = items0 + extra * (n_units - rem) + unit;
   }
-  const int item = items0 + extra * (units - rem) + unit + i * units;
-  return item < total ? item : -1;
-}
+  __device__ __forceinline__ int next() {
+    if (left == 0) {
+      if (extra_left > 0) {
+        at = extra_at;
+        step = extra_step;
+        left = extra_left;
+        extra_left = 0;
+      } else {
+        at = rest_at;
+        step = units;
+        left = 0x7FFFFFFF;
+      }
+    }
+    --left;
+    const int item = at;
+    if (item >= total) {
+      left = 1;  // stays behind the end
+      return -1;
+    }
+    at += step;
+    return item;
+  }
+};
 
 struct Item {
   int prob, m_blk, n_blk, split, kb0, nkb;
@@ -197,16 +235,14 @@ __device__ __forceinline__ Item decode(const Params& p, int item) {
   w.prob = item >= p.prob[0].items ? 1 : 0;
   const Problem& q = p.prob[w.prob];
   int t = w.prob ? item - p.prob[0].items : item;
-  const int tiles = q.m_blocks * q.n_blocks;
-  w.split = t / tiles;
-  t -= w.split * tiles;
-  const int span = q.raster_group * q.n_blocks;
-  const int group = t / span;
+  w.split = q.splits > 1 ? q.tiles.div(t) : 0;
+  t -= w.split * q.tiles.d;
+  const int group = q.span.div(t);
   const int first = group * q.raster_group;
-  const int rows = min(q.raster_group, q.m_blocks - first);
-  const int in_group = t - group * span;
-  w.m_blk = first + in_group % rows;
-  w.n_blk = in_group / rows;
+  const int in_group = t - group * q.span.d;
+  const FastDiv& rows = first + q.raster_group <= q.m_blocks ? q.group : q.last_group;
+  w.n_blk = rows.div(in_group);
+  w.m_blk = first + in_group - w.n_blk * rows.d;
   w.kb0 = w.split * q.kb_per_split;
   w.nkb = min(q.kb_per_split, q.num_kb - w.kb0);
   return w;
@@ -381,8 +417,8 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
     uint32_t phase = 0;
     long long issued = 0;
     bool ok = true;
-    for (int i = 0; ok; ++i) {
-      const int item = nth_item(p, unit, units, i);
+    for (Walk walk(p, unit, units); ok;) {
+      const int item = walk.next();
       if (item < 0) break;
       const Item w = decode(p, item);
       const Problem& q = p.prob[w.prob];
@@ -455,8 +491,8 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
       bool ok = true;
       const uint32_t desc_hi = smem_desc_hi_sw128();
       const uint32_t peer_delta = CG == 2 ? map_to_cta(bar_base, 1u) - bar_base : 0u;
-      for (int i = 0; ok; ++i) {
-        const int item = nth_item(p, unit, units, i);
+      for (Walk walk(p, unit, units); ok;) {
+        const int item = walk.next();
         if (item < 0) break;
         const Item w = decode(p, item);
         const Problem& q = p.prob[w.prob];
@@ -518,12 +554,12 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
     if constexpr (MODE == kProduct) unscale = __ldg(p.unscale);
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int i = 0;; ++i) {
-      const int item = nth_item(p, unit, units, i);
+    for (Walk walk(p, unit, units);;) {
+      const int item = walk.next();
       if (item < 0) break;
       const Item w = decode(p, item);
       const Problem& q = p.prob[w.prob];
-      if (!waiter.wait_relaxed(acc_full_bar(acc), acc_phase, gemm::kStatusEpilogueAccFullWait, item, 64u)) break;
+      if (!waiter.wait_relaxed(acc_full_bar(acc), acc_phase, gemm::kStatusEpilogueAccFullWait, item, w.nkb <= 4 ? 20u : 64u)) break;
       tc_fence_after_sync();
       const int row = w.m_blk * kTileM + row_in_tile;
       const bool row_ok = row < q.M;

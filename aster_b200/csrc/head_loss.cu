@@ -571,6 +571,10 @@ int set_items(Problem* q) {
   const int64_t items = static_cast<int64_t>(q->m_blocks) * q->n_blocks * q->splits;
   B200_REQUIRE(items < (1ll << 30), "head_loss: %lld tiles are more than one launch covers", (long long)items);
   q->items = static_cast<int>(items);
+  q->tiles = head::FastDiv::of(q->m_blocks * q->n_blocks);
+  q->span = head::FastDiv::of(q->raster_group * q->n_blocks);
+  q->group = head::FastDiv::of(q->raster_group);
+  q->last_group = head::FastDiv::of(q->m_blocks % q->raster_group != 0 ? q->m_blocks % q->raster_group : q->raster_group);
   return B200_OK;
 }
 

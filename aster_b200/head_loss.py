@@ -199,6 +199,13 @@ class _HeadLoss(torch.autograd.Function):
         return None if dx is None else dx.view(ctx.shape), dw, None, None
 
 
+def _apply(x: torch.Tensor, w: torch.Tensor, head: _Head, shape) -> torch.Tensor:
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+        return _HeadLoss.apply(x, w, head, shape)
+    loss = head.forward()[0]  # nothing to differentiate: no graph
+    return loss.view(shape) if head.per_row else loss
+
+
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100, label_smoothing: float = 0.0,
                          reduction: str = "mean", grad_bytes: int = 0) -> torch.Tensor:
     """Softmax cross entropy of ``x . weight^T`` against ``target``, as
@@ -209,8 +216,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     no gradient; any other target outside the vocabulary makes its loss, and the gradients it enters, NaN.
     "mean" divides by the number of targets that count (NaN without any).  ``grad_bytes`` limits what the
     backward pass keeps of ``dL/dz`` at a time (0: 256 MiB)."""
-    head = _xent_head(x, weight, target, ignore_index, label_smoothing, reduction, grad_bytes)
-    return _HeadLoss.apply(x, weight, head, target.shape)
+    return _apply(x, weight, _xent_head(x, weight, target, ignore_index, label_smoothing, reduction, grad_bytes), target.shape)
 
 
 def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor, *, temperature: float = 1.0,
@@ -223,8 +229,7 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: t
     order, ``top`` at most 1024.  Entries with a negative id or a logit of minus infinity are left out; rows with
     nothing left have no loss and no gradient and do not count for "mean".  An id listed twice counts twice; an
     id beyond the vocabulary, or a logit that is NaN or plus infinity, makes the row NaN."""
-    head = _distill_head(x, weight, teacher_logits, teacher_ids, temperature, reduction, grad_bytes)
-    return _HeadLoss.apply(x, weight, head, teacher_ids.shape[:-1])
+    return _apply(x, weight, _distill_head(x, weight, teacher_logits, teacher_ids, temperature, reduction, grad_bytes), teacher_ids.shape[:-1])
 
 
 def head_loss_status() -> Sequence[int]:
