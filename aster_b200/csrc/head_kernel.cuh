@@ -33,7 +33,10 @@ namespace head {
 using gemm::kBM;
 using gemm::kRowBytes;
 
-constexpr int kThreads = 192;
+// Epilogue warps: one per quarter of the TMEM lanes; two, each with half of a tile's columns, where a tile has so
+// few K blocks that its output decides (a warp's read of 64 columns takes 512 cycles, 16 bytes per cycle and
+// quarter, which the other warp's arithmetic then fills).
+constexpr int threads(int epilogue_warps) { return 64 + 32 * epilogue_warps; }
 constexpr int kStageK = 64;            // elements of K per stage (16-bit operands, 128 bytes)
 constexpr int kBoxBytes = 64 * kRowBytes;  // one box of an MN-major operand
 constexpr int kMaxStages = 16;
@@ -120,8 +123,8 @@ constexpr int kBarrierBytes = 384;
 // 4 KB per epilogue warp in which 32 rows x 128 bytes of output are turned around (a lane per row writes them,
 // eight lanes per row read them), so that they leave as whole lines.
 constexpr int kTurnBytes = 32 * 128;
-__host__ __device__ constexpr int smem_bytes(int bn, int stages, int cg, int am) {
-  return stages * stage_bytes(bn, cg, am) + gemm::kEpilogueWarps * kTurnBytes + overrun_bytes(bn, cg, am) + kBarrierBytes + 1024;
+__host__ __device__ constexpr int smem_bytes(int bn, int stages, int cg, int am, int epilogue_warps) {
+  return stages * stage_bytes(bn, cg, am) + epilogue_warps * kTurnBytes + overrun_bytes(bn, cg, am) + kBarrierBytes + 1024;
 }
 
 // 2^x for the softmax: the hardware's approximation (2 ulp) with results below 2^-126 flushed; the
@@ -341,13 +344,14 @@ __device__ __forceinline__ Labels labels_from(const Params& p, int row, bool row
   return l;
 }
 
-// T16: the 16-bit type of the operands, of G and of the gradients.
-template <int CG, int MODE, typename T16>
-__global__ void __launch_bounds__(kThreads, 1)
+// T16: the 16-bit type of the operands, of G and of the gradients.  EW: epilogue warps, 4 or (kProduct) 8.
+template <int CG, int MODE, typename T16, int EW>
+__global__ void __launch_bounds__(threads(EW), 1)
 head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_b0, const __grid_constant__ CUtensorMap map_a1,
             const __grid_constant__ CUtensorMap map_b1, const __grid_constant__ Params p) {
 #if defined(__CUDA_ARCH_FEAT_SM100_ALL)
   using namespace sm100;
+  static_assert(EW == 4 || (EW == 8 && MODE == kProduct), "a second epilogue warp per quarter: products only");
   constexpr int kTileM = kBM * CG;
   constexpr uint32_t kTmemCols = 2 * kMaxBn;
 
@@ -360,7 +364,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
   const uint32_t st_bytes = a_bytes + b_bytes;
   // (what a short A stage's 128-row read touches behind the ring is the turn-around buffers, and what follows them)
   [[maybe_unused]] const uint32_t turn_base = smem_base + static_cast<uint32_t>(p.stages) * st_bytes;
-  const uint32_t bar_base = turn_base + gemm::kEpilogueWarps * kTurnBytes + static_cast<uint32_t>(overrun_bytes(p.bn, CG, p.am));
+  const uint32_t bar_base = turn_base + EW * kTurnBytes + static_cast<uint32_t>(overrun_bytes(p.bn, CG, p.am));
   uint8_t* bar_ptr = smem_raw + (bar_base - smem_raw_u32);
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 128u + 8u * s; };
@@ -386,7 +390,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(acc_full_bar(a), 1);
-      mbar_init(acc_empty_bar(a), gemm::kEpilogueWarps * CG);
+      mbar_init(acc_empty_bar(a), EW * CG);
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0u;
@@ -549,6 +553,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
   } else {
     // ------------------------------- epilogue -------------------------------
     const int quarter = warp & 3;
+    [[maybe_unused]] const uint32_t turn_buf = turn_base + static_cast<uint32_t>(warp - 2) * kTurnBytes;
     const int row_in_tile = static_cast<int>(cta_rank) * kBM + quarter * 32 + lane;
     float unscale = 1.0f;
     if constexpr (MODE == kProduct) unscale = __ldg(p.unscale);
@@ -662,17 +667,19 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
           }
           // Rows of G are whole 64-column groups: what a piece writes behind the last column is never read.
           const bool col_ok = c + piece_col < cols;
-          turn_around(turn_base + static_cast<uint32_t>(quarter) * kTurnBytes, out, [&](int i, const uint4& t) {
+          turn_around(turn_buf, out, [&](int i, const uint4& t) {
             if (col_ok && piece_row + 4 * i < q.M) *reinterpret_cast<uint4*>(dst + static_cast<size_t>(4 * i) * p.g_ld + c) = t;
           });
         }
       } else {
         const int piece_row = row - lane + (lane >> 3);
+        const int half = EW == 8 ? (warp - 2) >> 2 : 0;
+        const int c_first = half * (kMaxBn / 2), c_end = !slab_ok ? 0 : (EW == 8 && half == 0 ? min(cols, kMaxBn / 2) : cols);
         if (q.out16 != nullptr) {
           const int piece_col = (lane & 7) * 8;
           T16* const dst = static_cast<T16*>(q.out16) + static_cast<size_t>(piece_row) * q.ld + tile_col + piece_col;
 #pragma unroll 1
-          for (int c = 0; c < (slab_ok ? cols : 0); c += 64) {
+          for (int c = c_first; c < c_end; c += 64) {
             uint32_t v[64];
             tmem_ld_32x32b_x64(taddr + static_cast<uint32_t>(c), v);
             tmem_ld_wait();
@@ -680,7 +687,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
 #pragma unroll
             for (int j = 0; j < 32; ++j) out[j] = pack2<T16>(__uint_as_float(v[2 * j]) * unscale, __uint_as_float(v[2 * j + 1]) * unscale);
             const bool col_ok = c + piece_col < cols;  // the columns are a multiple of 8: a piece exists or does not
-            turn_around(turn_base + static_cast<uint32_t>(quarter) * kTurnBytes, out, [&](int i, const uint4& t) {
+            turn_around(turn_buf, out, [&](int i, const uint4& t) {
               if (col_ok && piece_row + 4 * i < q.M) *reinterpret_cast<uint4*>(dst + static_cast<size_t>(4 * i) * q.ld + c) = t;
             });
           }
@@ -688,14 +695,14 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
           const int piece_col = (lane & 7) * 4;
           float* const dst = q.partial + (static_cast<size_t>(w.split) * q.M + piece_row) * q.N + tile_col + piece_col;
 #pragma unroll 1
-          for (int c = 0; c < (slab_ok ? cols : 0); c += 32) {
+          for (int c = c_first; c < c_end; c += 32) {
             uint32_t v[32];
             tmem_ld_32x32b_x32(taddr + static_cast<uint32_t>(c), v);
             tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * unscale);
             const bool col_ok = c + piece_col < cols;
-            turn_around(turn_base + static_cast<uint32_t>(quarter) * kTurnBytes, v, [&](int i, const uint4& t) {
+            turn_around(turn_buf, v, [&](int i, const uint4& t) {
               if (col_ok && piece_row + 4 * i < q.M) {
                 float4* const d = reinterpret_cast<float4*>(dst + static_cast<size_t>(4 * i) * q.N + c);
                 float4 f = make_float4(__uint_as_float(t.x), __uint_as_float(t.y), __uint_as_float(t.z), __uint_as_float(t.w));

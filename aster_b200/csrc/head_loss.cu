@@ -318,14 +318,15 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict_
 // ---------------------------------------------------------------------------------------------
 struct Tiling {
   int cg, bn, am, stages, smem;
+  int warps;  // epilogue warps
 };
 
 int ring(Tiling* t) {
-  const int room = kMaxSmem - head::kBarrierBytes - 1024 - gemm::kEpilogueWarps * head::kTurnBytes - head::overrun_bytes(t->bn, t->cg, t->am);
+  const int room = kMaxSmem - head::kBarrierBytes - 1024 - t->warps * head::kTurnBytes - head::overrun_bytes(t->bn, t->cg, t->am);
   // With few rows the product streams w from DRAM, which is fastest with about 112 KB of it on request per SM.
   const int cap = t->am < 128 ? std::max(4, 112 * 1024 / (t->bn * head::kRowBytes)) : 8;
   t->stages = std::min(cap, room / head::stage_bytes(t->bn, t->cg, t->am));
-  t->smem = head::smem_bytes(t->bn, t->stages, t->cg, t->am);
+  t->smem = head::smem_bytes(t->bn, t->stages, t->cg, t->am, t->warps);
   // One CTA per SM: each takes all of TMEM.
   if (t->smem <= kMaxSmem / 2) t->smem = kMaxSmem / 2 + 1024;
   return t->stages;
@@ -339,6 +340,7 @@ int choose_cg(int64_t tokens) { return div_up(tokens, 128) * 128 * 5 <= div_up(t
 // for a pair's 256 x 256, as long as its MMAs, and longer than them for everything narrower.
 Tiling z_tiling(int64_t tokens, int64_t cols) {
   Tiling t = {};
+  t.warps = 4;
   t.cg = choose_cg(tokens);
   t.am = t.cg == 1 && tokens <= 64 ? (tokens <= 32 ? 32 : 64) : 128;
   const int64_t units = kSms / t.cg, m_blocks = div_up(tokens, 128 * t.cg);
@@ -421,6 +423,9 @@ int make_plan(const b200_head_desc& d, Plan* p) {
   p->prod.cg = p->z.cg;
   p->prod.bn = 256;
   p->prod.am = 128;
+  // dW's tiles have tokens / 64 K blocks.  With two of them or fewer its output decides, and eight epilogue
+  // warps pay (8 x 4096 x 32768: backward 181 -> 168 us); with more they only take power from the MMAs (333 tokens: 50 -> 53 us).
+  p->prod.warps = p->prod.cg == 1 && d.tokens <= 128 ? 8 : 4;
   ring(&p->prod);
   // dX has few tiles with a long K (the range), dW many with a short one (the tokens).  dX is cut until a
   // part is at most half of what an SM does in all, which keeps the last round short.
@@ -450,9 +455,12 @@ int raster(int64_t m_blocks, int64_t tile_m, int64_t k) {
 using KernelFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap, const Params);
 
 template <int MODE>
-KernelFn kernel_for(int cg, int dtype) {
-  if (dtype == B200_F16) return cg == 2 ? head::head_kernel<2, MODE, __half> : head::head_kernel<1, MODE, __half>;
-  return cg == 2 ? head::head_kernel<2, MODE, __nv_bfloat16> : head::head_kernel<1, MODE, __nv_bfloat16>;
+KernelFn kernel_for(int cg, int dtype, int warps = 4) {
+  if constexpr (MODE == head::kProduct) {
+    if (warps == 8) return dtype == B200_F16 ? head::head_kernel<1, MODE, __half, 8> : head::head_kernel<1, MODE, __nv_bfloat16, 8>;
+  }
+  if (dtype == B200_F16) return cg == 2 ? head::head_kernel<2, MODE, __half, 4> : head::head_kernel<1, MODE, __half, 4>;
+  return cg == 2 ? head::head_kernel<2, MODE, __nv_bfloat16, 4> : head::head_kernel<1, MODE, __nv_bfloat16, 4>;
 }
 
 uint32_t idesc(int dtype, const Tiling& t, bool a_mn, bool b_mn) {
@@ -477,7 +485,7 @@ int init_device(int dev, DeviceState* st) {
   if (major != 10) return b200::fail(B200_ERR_NO_DEVICE, "device %d has compute capability %d.x; the kernels need sm_100", dev, major);
   for (int dtype : {B200_F16, B200_BF16}) {
     for (int cg : {1, 2}) {
-      for (KernelFn fn : {kernel_for<head::kStats>(cg, dtype), kernel_for<head::kGrad>(cg, dtype), kernel_for<head::kProduct>(cg, dtype)}) {
+      for (KernelFn fn : {kernel_for<head::kStats>(cg, dtype), kernel_for<head::kGrad>(cg, dtype), kernel_for<head::kProduct>(cg, dtype), kernel_for<head::kProduct>(1, dtype, 8)}) {
         B200_CUDA_OK(cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
       }
     }
@@ -510,7 +518,7 @@ int launch(KernelFn fn, const Tiling& t, Params* p, const CUtensorMap (&maps)[4]
   p->stages = t.stages;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(items, kSms / t.cg)) * t.cg);
-  cfg.blockDim = dim3(head::kThreads);
+  cfg.blockDim = dim3(static_cast<unsigned>(head::threads(t.warps)));
   cfg.dynamicSmemBytes = static_cast<size_t>(t.smem);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -813,7 +821,7 @@ int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const voi
       ++q.num_probs;
     }
     if (q.num_probs == 2) q.extra_rounds = std::max(1, q.prob[0].kb_per_split / q.prob[1].num_kb);
-    rc = launch(kernel_for<head::kProduct>(pl.prod.cg, d.dtype), pl.prod, &q, maps, s);
+    rc = launch(kernel_for<head::kProduct>(pl.prod.cg, d.dtype, pl.prod.warps), pl.prod, &q, maps, s);
     if (rc != B200_OK) return rc;
   }
   if (grad_x != nullptr && !pl.direct) {

@@ -245,6 +245,26 @@ class TestCrossEntropy:
             ref.check_loss(loss)
             ref.check_grads(*torch.autograd.grad(loss, (x, w)))
 
+    def test_offsets_beyond_32_bits(self, gpu):
+        """A stored range of dL/dz of more than 2^31 elements (4.4 GB) gives dW the bits that short ranges give it."""
+        T, D, V = 66000, 64, 33001
+        x, w, g = make(T, D, V, BF16, 19)
+        t = targets(T, V, g)
+        x.requires_grad_(), w.requires_grad_()
+        assert hl._sizes(hl._xent_head(x, w, t, -100, 0.0, "mean", 1 << 34).desc).grad_columns * T > 1 << 31
+        long = torch.autograd.grad(hl.linear_cross_entropy(x, w, t, grad_bytes=1 << 34), (x, w))
+        short = torch.autograd.grad(hl.linear_cross_entropy(x, w, t), (x, w))
+        assert torch.equal(long[1], short[1])
+        # dX: another order of the same sums (fp32 roundings), rounded to bf16
+        difference = (long[0].double() - short[0].double()).abs()
+        assert bool((difference <= 2.0 ** -7 * short[0].double().abs() + 2.0 ** -15 * short[0].double().abs().max()).all())
+        rows = torch.tensor([0, T - 1, T // 2, 65535], device="cuda")
+        q = torch.softmax(x.detach()[rows].double() @ w.detach().double().T, 1)
+        kept = t[rows] >= 0
+        q[torch.nonzero(kept)[:, 0], t[rows][kept]] -= 1
+        want = torch.where(kept[:, None], q @ w.detach().double() / (t >= 0).sum(), 0.0)
+        assert bool(((long[0][rows].double() - want).abs() <= 2.0 ** -6 * want.abs().max()).all())
+
     def test_against_differences(self, gpu):
         x, w, g = make(40, 64, 300, F16, 7)
         t = targets(40, 300, g)

@@ -163,6 +163,17 @@ class TestQuantizeOnGpu:
             want = top.quantize_mx_direct(view.contiguous().clone())
             assert torch.equal(q, want[0]) and torch.equal(s, want[1])
 
+    def test_offsets_beyond_32_bits(self, gpu):
+        rows, K = 265000, 8192  # 2.17e9 values
+        x = torch.randn(rows, K, device="cuda", dtype=torch.bfloat16)
+        q, s = top.quantize_mx_direct(x)
+        tail = 128 * 3
+        first = rows // 128 * 128 - tail
+        q2, s2 = top.quantize_mx_direct(x[first:])
+        assert torch.equal(q[first:], q2) and torch.equal(s[-s2.numel():], s2)
+        y = top.dequantize_mx_direct(q, s, torch.bfloat16)
+        assert torch.equal(y[first:], top.dequantize_mx_direct(q2, s2, torch.bfloat16))
+
     def test_refusals(self, gpu):
         x = torch.zeros(4, 64, device="cuda")
         for bad in (x[:, :48], x[:0], x.double(), x[0], x[:, :0]):
