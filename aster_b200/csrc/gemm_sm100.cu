@@ -42,6 +42,19 @@ EncodeTiledFn encode_tiled_fn() {
   return fn;
 }
 
+// The encoder is a driver call and needs a context that is current on the calling thread.  The runtime binds
+// one with the thread's first launch or allocation; a thread whose first call is this one (an autograd
+// worker's backward pass) has none yet, and cudaSetDevice binds it.
+template <typename... Args>
+CUresult encode_tiled(EncodeTiledFn fn, Args... args) {
+  CUresult r = fn(args...);
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = fn(args...);
+  }
+  return r;
+}
+
 }  // namespace
 
 // Row-major [rows, cols] matrix of `elt_bytes`-wide elements, tiled in boxes of
@@ -65,7 +78,7 @@ int b200::make_strided_operand_map(CUtensorMap* map, const void* base, int dtype
   cuuint64_t strides[1] = {row_stride * eb};
   cuuint32_t box[2] = {static_cast<cuuint32_t>(gemm::kRowBytes / eb), box_rows};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  CUresult r = encode_tiled(fn, map, dt, 2u, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     return b200::fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (rows=%llu cols=%llu box_rows=%u)",
@@ -87,7 +100,7 @@ int make_scale_map(CUtensorMap* map, const void* base, uint64_t blocks, uint32_t
   cuuint64_t strides[1] = {gemm::kScaleBlockBytes};
   cuuint32_t box[2] = {gemm::kScaleBlockBytes / 4, per_copy};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  CUresult r = encode_tiled(fn, map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2u, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return b200::fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (%llu scale blocks)", static_cast<int>(r), (unsigned long long)blocks);
   return B200_OK;

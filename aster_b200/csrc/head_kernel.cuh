@@ -106,12 +106,17 @@ struct Params {
   uint32_t* ticket;        // cleared for the reduction that follows
   // kGrad
   const float* lse;        // [tokens]
-  const float* coef;       // [tokens]
+  const float* coef;       // [tokens] row factors; null: `coef_top` for every row that has a loss
+  float coef_top;
+  const float* weight;     // distillation: [tokens] 1, 0 (no loss) or NaN
   float base;              // smoothing / vocab
   void* g;                 // [tokens][g_ld]
   int64_t g_ld;
   // kProduct
-  const float* unscale;    // one factor on everything
+  const float* unscale;    // one factor on everything; null: *share * *grad_loss * unscale_factor
+  const float* share;
+  const float* grad_loss;
+  float unscale_factor;
 };
 
 __host__ __device__ constexpr int stage_bytes(int bn, int cg, int am) { return (am + bn / cg) * kRowBytes; }
@@ -311,6 +316,13 @@ struct Labels {
 __device__ __forceinline__ int target_class(const Params& p, int row) {
   const long long t = p.target64 ? __ldg(static_cast<const long long*>(p.target) + row) : static_cast<long long>(__ldg(static_cast<const int*>(p.target) + row));
   return t != p.ignore_index && t >= 0 && t < p.vocab ? static_cast<int>(t) : kNoLabel;
+}
+
+// 1 for a row with a loss, 0 for one without, NaN for one with a bad label.
+__device__ __forceinline__ float row_weight(const Params& p, int row) {
+  if (p.weight != nullptr) return __ldg(p.weight + row);
+  const long long t = p.target64 ? __ldg(static_cast<const long long*>(p.target) + row) : static_cast<long long>(__ldg(static_cast<const int*>(p.target) + row));
+  return t == p.ignore_index ? 0.0f : (t >= 0 && t < p.vocab ? 1.0f : NAN);
 }
 
 // Labels of `row` from column `col` on.
@@ -556,7 +568,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
     [[maybe_unused]] const uint32_t turn_buf = turn_base + static_cast<uint32_t>(warp - 2) * kTurnBytes;
     const int row_in_tile = static_cast<int>(cta_rank) * kBM + quarter * 32 + lane;
     float unscale = 1.0f;
-    if constexpr (MODE == kProduct) unscale = __ldg(p.unscale);
+    if constexpr (MODE == kProduct) unscale = p.unscale != nullptr ? __ldg(p.unscale) : __ldg(p.share) * __ldg(p.grad_loss) * p.unscale_factor;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (Walk walk(p, unit, units);;) {
@@ -630,7 +642,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
       } else if constexpr (MODE == kGrad) {
         const int vcol = p.col0 + tile_col;
         Labels l = labels_from(p, row, row_ok, vcol);
-        const float coef = row_ok ? __ldg(p.coef + row) : 0.0f;
+        const float coef = !row_ok ? 0.0f : (p.coef != nullptr ? __ldg(p.coef + row) : p.coef_top * row_weight(p, row));
         const float lse2 = row_ok ? __ldg(p.lse + row) * 1.4426950408889634f : 0.0f;
         const float shift = coef * p.base;
         const int piece_row = row - lane + (lane >> 3), piece_col = (lane & 7) * 8;  // of every 4 rows, of every 64 columns

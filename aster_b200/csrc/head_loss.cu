@@ -30,6 +30,7 @@ constexpr int kSms = 148;
 constexpr int kMaxSmem = 232448;
 constexpr int64_t kGradBytes = 256ll << 20;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kHalfTop = 8192.0f;  // largest row factor of fp16's dL/dz
 
 __device__ uint32_t g_status[head::kStatusWords];
 
@@ -259,24 +260,23 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) 
     }
     const bool mean = p.reduction == B200_REDUCE_MEAN;
     *p.loss = static_cast<float>(mean ? a / k : a);
-    *p.share = mean ? static_cast<float>(1.0 / k) : 1.0f;
+    *p.share = !mean ? 1.0f : (k > 0.0 ? static_cast<float>(1.0 / k) : 0.0f);  // without any row the gradients are zero
   }
 }
 
 // Row factors c_t = dL/dL_t * dL_t/d(softmax - labels), 0 for rows without a loss, divided by the largest
-// of them: G = c_t (softmax - labels) is rounded to 16 bits, and with equal factors (mean, sum) its
-// entries at the labels are then close to 1 and -- nearly -- exact.  (Under the plain factor 1/N all of
-// them carried the one rounding error of 1/N: the gradients were off by 0.0035 instead of 0.0017, which
-// is the rounding of the result.)  fp16: the largest factor is 2^13, so that small probabilities keep
-// their digits, too.  `unscale` takes the divisor out of the gradients again, in fp32.
-__global__ void __launch_bounds__(1024) factor_kernel(const float* __restrict__ grad_loss, int per_row, const float* __restrict__ share, float row_scale,
-                                                      const void* __restrict__ target, int index_bits, long long ignore_index, int vocab,
-                                                      const float* __restrict__ weight, int tokens, int half_range, float* __restrict__ coef,
-                                                      float* __restrict__ unscale) {
+// of them: G = c_t (softmax - labels) is rounded to 16 bits, and with equal factors its entries at the labels
+// are then close to 1 and -- nearly -- exact.  (Under the plain factor 1/N all of them carried the one rounding
+// error of 1/N: the gradients were off by 0.0035 instead of 0.0017, which is the rounding of the result.)
+// fp16: the largest factor is 2^13, so that small probabilities keep their digits, too.  `unscale` takes the
+// divisor out of the gradients again, in fp32.  Mean and sum have equal factors and need no launch for this:
+// the row's own 1, 0 or NaN is its factor, and everything else is in the divisor.
+__global__ void __launch_bounds__(1024) factor_kernel(const float* __restrict__ grad_loss, float row_scale, const void* __restrict__ target, int index_bits,
+                                                      long long ignore_index, int vocab, const float* __restrict__ weight, int tokens, float top,
+                                                      float* __restrict__ coef, float* __restrict__ unscale) {
   __shared__ float buf[32];
   sm100::griddep_launch_dependents();
   sm100::griddep_wait();
-  const float sh = *share;
   auto factor = [&](int t) -> float {
     float w;
     if (weight != nullptr) {
@@ -285,9 +285,8 @@ __global__ void __launch_bounds__(1024) factor_kernel(const float* __restrict__ 
       const long long y = load_index(target, index_bits, t);
       w = y == ignore_index ? 0.0f : (y >= 0 && y < vocab ? 1.0f : NAN);
     }
-    return w == 0.0f ? 0.0f : w * row_scale * (sh * grad_loss[per_row ? t : 0]);
+    return w == 0.0f ? 0.0f : w * row_scale * grad_loss[t];
   };
-  const float top = half_range ? 8192.0f : 1.0f;
   float mx = 0.0f;
   for (int t = threadIdx.x; t < tokens; t += blockDim.x) {
     const float c = fabsf(factor(t));
@@ -738,10 +737,15 @@ int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const voi
   float* unscale = reinterpret_cast<float*>(ws + pl.b_unscale);
   float* parts = reinterpret_cast<float*>(ws + pl.b_parts);
   void* g = ws + pl.b_g;
-  rc = launch_small(factor_kernel, 1u, 1024u, s, grad_loss, d.reduction == B200_REDUCE_NONE, reinterpret_cast<const float*>(sv), distill ? d.temperature : 1.0f, labels,
-                    d.index_bits, d.ignore_index, static_cast<int>(d.vocab), distill ? reinterpret_cast<const float*>(sv + pl.s_weight) : nullptr,
-                    static_cast<int>(d.tokens), d.dtype == B200_F16, coef, unscale);
-  if (rc != B200_OK) return rc;
+  const bool per_row = d.reduction == B200_REDUCE_NONE;
+  const float row_scale = distill ? d.temperature : 1.0f, coef_top = d.dtype == B200_F16 ? kHalfTop : 1.0f;
+  const float* weight = distill ? reinterpret_cast<const float*>(sv + pl.s_weight) : nullptr;
+  const float* share = reinterpret_cast<const float*>(sv);
+  if (per_row) {
+    rc = launch_small(factor_kernel, 1u, 1024u, s, grad_loss, row_scale, labels, d.index_bits, d.ignore_index, static_cast<int>(d.vocab), weight,
+                      static_cast<int>(d.tokens), coef_top, coef, unscale);
+    if (rc != B200_OK) return rc;
+  }
 
   CUtensorMap z_maps[4] = {};
   rc = b200::make_strided_operand_map(&z_maps[0], x, d.dtype, d.tokens, d.hidden, d.x_stride, static_cast<uint32_t>(pl.grad.am));
@@ -763,7 +767,9 @@ int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const voi
     if (rc != B200_OK) return rc;
     p.col0 = static_cast<int>(col0);
     p.lse = lse;
-    p.coef = coef;
+    p.coef = per_row ? coef : nullptr;
+    p.coef_top = coef_top;
+    p.weight = weight;
     p.g = g;
     p.g_ld = pl.g_ld;
     rc = launch(kernel_for<head::kGrad>(pl.grad.cg, d.dtype), pl.grad, &p, z_maps, s);
@@ -774,7 +780,10 @@ int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const voi
     Params q;
     std::memset(&q, 0, sizeof(q));
     q.status = status;
-    q.unscale = unscale;
+    q.unscale = per_row ? unscale : nullptr;
+    q.share = share;
+    q.grad_loss = grad_loss;
+    q.unscale_factor = row_scale / coef_top;
     CUtensorMap maps[4] = {};
     if (grad_x != nullptr) {
       Problem& dx = q.prob[q.num_probs];

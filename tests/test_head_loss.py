@@ -426,6 +426,33 @@ class TestCrossEntropy:
         want = torch.autograd.grad(call(), (x, w))
         assert torch.equal(dx, want[0]) and torch.equal(dw, want[1])
 
+    def test_from_other_threads(self, gpu):
+        """Threads whose first CUDA call is the loss, or its backward pass, all at once."""
+        import threading
+
+        problems = [make(60 + i, 64, 900, BF16, 40 + i) for i in range(4)]
+        labels = [targets(60 + i, 900, p[2]) for i, p in enumerate(problems)]
+        leaves = [(p[0].requires_grad_(), p[1].requires_grad_()) for p in problems]
+        want = [torch.autograd.grad(hl.linear_cross_entropy(*l, t), l) for l, t in zip(leaves, labels)]
+        torch.cuda.synchronize()
+        got, errors = {}, []
+
+        def work(i):
+            try:
+                for _ in range(10):
+                    got[i] = torch.autograd.grad(hl.linear_cross_entropy(*leaves[i], labels[i]), leaves[i])
+                torch.cuda.synchronize()
+            except Exception as e:
+                errors.append(e)
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not errors
+        assert all(torch.equal(a, b) for i in range(4) for a, b in zip(got[i], want[i]))
+
     def test_operator_of_the_dispatcher(self, gpu):
         x, w, g = make(50, 64, 400, BF16, 16)
         t = targets(50, 400, g)

@@ -314,6 +314,30 @@ class TestProductOnGpu:
             with pytest.raises(RuntimeError):
                 top.gemm_mx_nt_direct(*args)
 
+    def test_from_other_threads(self, gpu):
+        """A thread whose first CUDA call is the product, and several that share one plan."""
+        import threading
+
+        pairs = [top.quantize_mx_direct(torch.randn(40, 256, device="cuda")) + top.quantize_mx_direct(torch.randn(72, 256, device="cuda")) for _ in range(4)]
+        want = [top.gemm_mx_nt_direct(*p) for p in pairs]
+        torch.cuda.synchronize()
+        got, errors = {}, []
+
+        def work(i):
+            try:
+                got[i] = [top.gemm_mx_nt_direct(*pairs[i]) for _ in range(50)]
+                torch.cuda.synchronize()
+            except Exception as e:
+                errors.append(e)
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not errors
+        assert all(torch.equal(c, want[i]) for i in range(4) for c in got[i])
+
     def test_graph_replay(self, gpu):
         """A captured quantise + product reads its inputs anew on each replay."""
         x, w = torch.randn(48, 512, device="cuda").bfloat16(), torch.randn(96, 512, device="cuda").bfloat16()
