@@ -42,6 +42,28 @@ struct Raw {
   uint32_t w[kPerLane * sizeof(T) / 4];
 };
 
+// Largest magnitude of the 8 values as fp32 bits (magnitudes compare as integers; infinities and NaN come out
+// largest), still within the lane; and the maximum over the 4 lanes of a block.
+__device__ __forceinline__ uint32_t block_max(uint32_t m) {
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+}
+__device__ __forceinline__ uint32_t amax_bits(const Raw<float>& r) {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) m = max(m, r.w[i] & 0x7FFFFFFFu);
+  return block_max(m);
+}
+// Two 16-bit magnitudes at a time.
+__device__ __forceinline__ uint32_t amax_16(const uint32_t (&w)[kPerLane / 2]) {
+  uint32_t m = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+  for (int i = 1; i < kPerLane / 2; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+  return block_max(max(m & 0xFFFFu, m >> 16));
+}
+__device__ __forceinline__ uint32_t amax_bits(const Raw<__nv_bfloat16>& r) { return amax_16(r.w) << 16; }
+__device__ __forceinline__ uint32_t amax_bits(const Raw<__half>& r) { return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(amax_16(r.w))))); }
+
 template <typename T>
 __device__ __forceinline__ float value(const Raw<T>& r, int i);
 template <>
@@ -141,15 +163,7 @@ __global__ void __launch_bounds__(kThreads) quantize_mx4_kernel(const T* __restr
 #pragma unroll
   for (int a = 0; a < kRows; ++a) {
     const int r = warp_row(t, a);
-    float v[kPerLane];
-    uint32_t amax = 0u;  // magnitudes compare as integers; infinities and NaN come out largest
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      v[i] = value<T>(raw[a], i);
-      amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    }
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const uint32_t amax = amax_bits(raw[a]);
     const uint32_t field = amax >> 23;  // biased exponent of the maximum; 0 below 2^-126
     uint32_t byte = field > 2u ? field - 2u : 0u;
     if (amax == 0u) byte = 127u;
@@ -158,7 +172,7 @@ __global__ void __launch_bounds__(kThreads) quantize_mx4_kernel(const T* __restr
     const float inv = __uint_as_float((254u - (bad ? 127u : byte)) << 23);
     uint32_t codes = 0u;
 #pragma unroll
-    for (int i = 0; i < kPerLane / 2; ++i) codes |= e2m1_pair(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
+    for (int i = 0; i < kPerLane / 2; ++i) codes |= e2m1_pair(value<T>(raw[a], 2 * i) * inv, value<T>(raw[a], 2 * i + 1) * inv) << (8 * i);
     if (bad) codes = 0u;
     if (r < t.rows && k_ok) *reinterpret_cast<uint32_t*>(dst + r * (K / 2)) = codes;
     uint32_t word = byte << (8 * ((lane >> 2) & 3));
