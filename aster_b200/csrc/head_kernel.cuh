@@ -269,46 +269,80 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Turns the warp's 32 rows x 128 bytes around: lane l brings row l as 32 words and gets 16-byte pieces of
-// rows 4 i + l / 8, piece l % 8, for i = 0..7, handed to `use(i, piece)`.
-template <typename Use>
-__device__ __forceinline__ void turn_around(uint32_t buf, const uint32_t (&w)[32], Use use) {
-  const uint32_t lane = threadIdx.x & 31;
-  const uint32_t wr = buf + lane * 128u, wr_swz = (lane & 7u) << 4;
-  __syncwarp();  // the previous pieces have been read
+// A warp's 32 rows x 128 bytes on their way from a lane per row to whole lines: lane l writes row l (16-byte
+// piece j at position j ^ (l % 8)) and reads pieces of rows 4 i + l / 8, piece l % 8, for i = 0..7.
+struct TurnAround {
+  uint32_t buf;
+
+  __device__ __forceinline__ uint32_t piece(uint32_t row, uint32_t j) const { return buf + row * 128u + ((j ^ (row & 7u)) << 4); }
+  // Pieces [first, first + N / 4) of this lane's row.  The first call of a round waits for the previous round's reads.
+  template <int N>
+  __device__ __forceinline__ void put(int first, const uint32_t (&w)[N]) const {
+    const uint32_t lane = threadIdx.x & 31;
+    if (first == 0) __syncwarp();
 #pragma unroll
-  for (uint32_t j = 0; j < 8; ++j) sm100::st_shared_u4(wr + ((j << 4) ^ wr_swz), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-  __syncwarp();
-  uint4 t[8];  // all reads before the first use: their latencies overlap
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t r = 4u * i + (lane >> 3);
-    t[i] = sm100::ld_shared_u4(buf + r * 128u + (((lane & 7u) ^ (r & 7u)) << 4));
+    for (int j = 0; j < N / 4; ++j) sm100::st_shared_u4(piece(lane, first + j), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
   }
+  // Element `at` (16 bits) of this lane's row, after its piece has been put.
+  __device__ __forceinline__ void patch16(int at, uint32_t bits) const {
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(piece(threadIdx.x & 31, at >> 3) + 2u * (at & 7)), "h"(static_cast<unsigned short>(bits)) : "memory");
+  }
+  // Element `at` (32 bits) of this lane's row.
+  __device__ __forceinline__ float own32(int at) const {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(piece(threadIdx.x & 31, at >> 2) + 4u * (at & 3)) : "memory");
+    return v;
+  }
+  template <typename Use>
+  __device__ __forceinline__ void get(Use use) const {
+    const uint32_t lane = threadIdx.x & 31;
+    __syncwarp();
+    uint4 t[8];  // all reads before the first use: their latencies overlap
 #pragma unroll
-  for (int i = 0; i < 8; ++i) use(i, t[i]);
+    for (int i = 0; i < 8; ++i) t[i] = sm100::ld_shared_u4(piece(4u * i + (lane >> 3), lane & 7u));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) use(i, t[i]);
+  }
+};
+
+// x[at] by halving: five selects deep.
+__device__ __forceinline__ float pick(const float (&x)[32], int at) {
+  float a[16], b[8], c[4];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) a[j] = at & 16 ? x[j + 16] : x[j];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) b[j] = at & 8 ? a[j + 8] : a[j];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c[j] = at & 4 ? b[j + 4] : b[j];
+  const float d = at & 2 ? c[2] : c[0], e = at & 2 ? c[3] : c[1];
+  return at & 1 ? e : d;
 }
 
-// A row's labels during the walk over a tile's columns, in rising order.
+// A row's labels during the walk over a tile's columns, in rising order.  The entry behind the next one is
+// fetched ahead: the lists of a tile's rows do not fit what the ring leaves of the L1, and a label should not
+// wait for the L2.
 struct Labels {
   const int32_t* ids;  // null: one label (cross entropy)
   const float* probs;
   int top, at;
-  int next;    // the next label's column, kNoLabel: none left
-  float prob;
+  int next, ahead;     // the next label's column and the one behind it, kNoLabel: none left
+  float prob, prob_ahead;
 
-  __device__ __forceinline__ void load() {
-    if (ids == nullptr) return;
+  __device__ __forceinline__ void fetch_ahead() {
+    const bool more = at + 1 < top;
+    ahead = more ? __ldg(ids + at + 1) : kNoLabel;
+    prob_ahead = more ? __ldg(probs + at + 1) : 0.0f;
+  }
+  __device__ __forceinline__ void start() {
     next = at < top ? __ldg(ids + at) : kNoLabel;
     prob = at < top ? __ldg(probs + at) : 0.0f;
+    fetch_ahead();
   }
   __device__ __forceinline__ void advance() {
     ++at;
-    if (ids == nullptr) {
-      next = kNoLabel;
-    } else {
-      load();
-    }
+    next = ahead;
+    prob = prob_ahead;
+    if (ids != nullptr) fetch_ahead();
   }
 };
 
@@ -332,8 +366,9 @@ __device__ __forceinline__ Labels labels_from(const Params& p, int row, bool row
   l.probs = nullptr;
   l.top = p.top;
   l.at = 0;
-  l.next = kNoLabel;
+  l.next = l.ahead = kNoLabel;
   l.prob = p.label_prob;
+  l.prob_ahead = 0.0f;
   if (!row_ok) return l;
   if (p.ids == nullptr) {
     const int t = target_class(p, row);
@@ -342,17 +377,23 @@ __device__ __forceinline__ Labels labels_from(const Params& p, int row, bool row
   }
   l.ids = p.ids + static_cast<size_t>(row) * p.top;
   l.probs = p.probs + static_cast<size_t>(row) * p.top;
-  int lo = 0, hi = p.top;  // first entry at or behind `col`
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(l.ids + mid) < col) {
-      lo = mid + 1;
-    } else {
-      hi = mid;
+  // First entry at or behind `col`, by eighths: the eight probes of a round are independent loads, so that 64
+  // entries take two trips to the L2 instead of six.
+  int lo = 0, n = p.top;
+  while (n > 0) {
+    const int step = (n + 7) >> 3, end = lo + n;
+    int below = 0;
+#pragma unroll
+    for (int i = 1; i <= 8; ++i) {
+      const int at = lo + i * step - 1;
+      below += at < end && __ldg(l.ids + at) < col ? 1 : 0;
     }
+    lo += below * step;  // the last entry of the next eighth is at or behind `col`
+    lo = min(lo, end);
+    n = min(step - 1, end - lo);
   }
   l.at = lo;
-  l.load();
+  l.start();
   return l;
 }
 
@@ -565,7 +606,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
   } else {
     // ------------------------------- epilogue -------------------------------
     const int quarter = warp & 3;
-    [[maybe_unused]] const uint32_t turn_buf = turn_base + static_cast<uint32_t>(warp - 2) * kTurnBytes;
+    [[maybe_unused]] const TurnAround turn{turn_base + static_cast<uint32_t>(warp - 2) * kTurnBytes};
     const int row_in_tile = static_cast<int>(cta_rank) * kBM + quarter * 32 + lane;
     float unscale = 1.0f;
     if constexpr (MODE == kProduct) unscale = p.unscale != nullptr ? __ldg(p.unscale) : __ldg(p.share) * __ldg(p.grad_loss) * p.unscale_factor;
@@ -576,17 +617,26 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
       if (item < 0) break;
       const Item w = decode(p, item);
       const Problem& q = p.prob[w.prob];
-      if (!waiter.wait_relaxed(acc_full_bar(acc), acc_phase, gemm::kStatusEpilogueAccFullWait, item, w.nkb <= 4 ? 20u : 64u)) break;
-      tc_fence_after_sync();
       const int row = w.m_blk * kTileM + row_in_tile;
       const bool row_ok = row < q.M;
+      // What the row needs, and the search for the tile's first label, come while the tile's MMAs run.
+      [[maybe_unused]] Labels l;
+      if constexpr (MODE != kProduct) l = labels_from(p, row, row_ok, p.col0 + w.n_blk * p.bn);
+      [[maybe_unused]] float coef = 0.0f, lse2 = 0.0f;
+      if constexpr (MODE == kGrad) {
+        if (row_ok) {
+          coef = p.coef != nullptr ? __ldg(p.coef + row) : p.coef_top * row_weight(p, row);
+          lse2 = __ldg(p.lse + row) * 1.4426950408889634f;
+        }
+      }
+      if (!waiter.wait_relaxed(acc_full_bar(acc), acc_phase, gemm::kStatusEpilogueAccFullWait, item, w.nkb <= 4 ? 20u : 64u)) break;
+      tc_fence_after_sync();
       const bool slab_ok = row - lane < q.M;  // does any of the warp's rows exist?
       const int tile_col = w.n_blk * p.bn;    // in the columns of this launch
       const int cols = min(p.bn, q.N - tile_col);
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kMaxBn);
       if constexpr (MODE == kStats) {
         float m = -INFINITY, s = 0.0f, zsum = 0.0f;
-        Labels l = labels_from(p, row, row_ok, tile_col);
 #pragma unroll 1
         for (int c = 0; c < (slab_ok ? cols : 0); c += 32) {
           uint32_t v[32];
@@ -622,13 +672,14 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
           s = fmaf(s, ex2(fmaf(m, p.scale2, -m2)), t0 + t1);
           m = nm;
           const int end = tile_col + c + 32;
-          while (__any_sync(0xffffffffu, l.next < end)) {
-            if (l.next < end) {
-              const int at = l.next - (tile_col + c);
-              float z = x[0];
+          if (__any_sync(0xffffffffu, l.next < end)) {
+            // Registers cannot be indexed: the lane's 32 logits go through its row of shared memory.
+            uint32_t zs[32];
 #pragma unroll
-              for (int j = 1; j < 32; ++j) z = at == j ? x[j] : z;
-              p.label_z[static_cast<size_t>(row) * p.top + l.at] = z;
+            for (int j = 0; j < 32; ++j) zs[j] = __float_as_uint(x[j]);
+            turn.put(0, zs);
+            while (l.next < end) {
+              p.label_z[static_cast<size_t>(row) * p.top + l.at] = turn.own32(l.next - (tile_col + c));
               l.advance();
             }
             __syncwarp();
@@ -641,9 +692,6 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
         }
       } else if constexpr (MODE == kGrad) {
         const int vcol = p.col0 + tile_col;
-        Labels l = labels_from(p, row, row_ok, vcol);
-        const float coef = !row_ok ? 0.0f : (p.coef != nullptr ? __ldg(p.coef + row) : p.coef_top * row_weight(p, row));
-        const float lse2 = row_ok ? __ldg(p.lse + row) * 1.4426950408889634f : 0.0f;
         const float shift = coef * p.base;
         const int piece_row = row - lane + (lane >> 3), piece_col = (lane & 7) * 8;  // of every 4 rows, of every 64 columns
         T16* const dst = static_cast<T16*>(p.g) + static_cast<size_t>(piece_row) * p.g_ld + tile_col + piece_col;
@@ -652,7 +700,6 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
           uint32_t v[64];
           tmem_ld_32x32b_x64(taddr + static_cast<uint32_t>(c), v);
           tmem_ld_wait();
-          uint32_t out[32];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float x[32];
@@ -662,24 +709,31 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
 #pragma unroll
               for (int j = 0; j < 32; ++j) x[j] = 0.0f;
             }
+            uint32_t out[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) out[j] = pack2<T16>(x[2 * j], x[2 * j + 1]);
+            turn.put(4 * h, out);
+            // The few entries at labels are taken out of the 32, corrected (an id may be listed more than once)
+            // and written over the rounded ones: cheaper than touching all 32 for each of them (4096 x 1024 x 16384
+            // with 64 labels per row: 159 -> 137 us; 105 with one label).
             const int col = vcol + c + 32 * h;
             const int end = c + 32 * h < cols ? col + 32 : 0;  // a tile may end after the first half
             while (__any_sync(0xffffffffu, l.next < end)) {
               if (l.next < end) {
-                const int at = l.next - col;
-                const float d = coef * l.prob;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) x[j] -= at == j ? d : 0.0f;
-                l.advance();
+                const int id = l.next;
+                float g = pick(x, id - col);
+                do {
+                  g -= coef * l.prob;
+                  l.advance();
+                } while (l.next == id);
+                turn.patch16(32 * h + id - col, pack2<T16>(g, 0.0f));
               }
               __syncwarp();
             }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) out[16 * h + j] = pack2<T16>(x[2 * j], x[2 * j + 1]);
           }
           // Rows of G are whole 64-column groups: what a piece writes behind the last column is never read.
           const bool col_ok = c + piece_col < cols;
-          turn_around(turn_buf, out, [&](int i, const uint4& t) {
+          turn.get([&](int i, const uint4& t) {
             if (col_ok && piece_row + 4 * i < q.M) *reinterpret_cast<uint4*>(dst + static_cast<size_t>(4 * i) * p.g_ld + c) = t;
           });
         }
@@ -699,7 +753,8 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
 #pragma unroll
             for (int j = 0; j < 32; ++j) out[j] = pack2<T16>(__uint_as_float(v[2 * j]) * unscale, __uint_as_float(v[2 * j + 1]) * unscale);
             const bool col_ok = c + piece_col < cols;  // the columns are a multiple of 8: a piece exists or does not
-            turn_around(turn_buf, out, [&](int i, const uint4& t) {
+            turn.put(0, out);
+            turn.get([&](int i, const uint4& t) {
               if (col_ok && piece_row + 4 * i < q.M) *reinterpret_cast<uint4*>(dst + static_cast<size_t>(4 * i) * q.ld + c) = t;
             });
           }
@@ -714,7 +769,8 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * unscale);
             const bool col_ok = c + piece_col < cols;
-            turn_around(turn_buf, v, [&](int i, const uint4& t) {
+            turn.put(0, v);
+            turn.get([&](int i, const uint4& t) {
               if (col_ok && piece_row + 4 * i < q.M) {
                 float4* const d = reinterpret_cast<float4*>(dst + static_cast<size_t>(4 * i) * q.N + c);
                 float4 f = make_float4(__uint_as_float(t.x), __uint_as_float(t.y), __uint_as_float(t.z), __uint_as_float(t.w));

@@ -70,53 +70,71 @@ __device__ __forceinline__ long long load_index(const void* p, int bits, size_t 
   return bits == 64 ? __ldg(static_cast<const long long*>(p) + i) : static_cast<long long>(__ldg(static_cast<const int*>(p) + i));
 }
 
-// One block per row: the teacher's probabilities over its listed entries, sorted by id (each entry's
-// place is the number of entries before it, ties in listing order: no two write the same place).
-__global__ void __launch_bounds__(256) teacher_kernel(const void* __restrict__ logits, int dtype, const void* __restrict__ ids_in, int bits, int top,
-                                                      int vocab, float inv_t, int32_t* __restrict__ ids, float* __restrict__ probs,
-                                                      float* __restrict__ weight, float* __restrict__ neg_entropy) {
-  __shared__ int32_t s_id[kMaxTop];
-  __shared__ float s_t[kMaxTop];
+// One block per row: the teacher's probabilities over its listed entries, sorted by id (a bitonic network over
+// the next power of two `n`; the key's low half is the listing order, so that equal ids stay in it and no two
+// keys are equal).
+__global__ void __launch_bounds__(kMaxTop / 2) teacher_kernel(const void* __restrict__ logits, int dtype, const void* __restrict__ ids_in, int bits, int top, int n,
+                                                              int vocab, float inv_t, int32_t* __restrict__ ids, float* __restrict__ probs,
+                                                              float* __restrict__ weight, float* __restrict__ neg_entropy) {
+  extern __shared__ uint64_t key[];  // [n], then [n] floats: as little as the rows need, so that an SM holds 32 of them
+  float* const s_t = reinterpret_cast<float*>(key + n);
   __shared__ float buf[32];
   const size_t row = blockIdx.x, base = row * top;
   sm100::griddep_launch_dependents();
   sm100::griddep_wait();
-  float mx = -INFINITY, any = 0.0f, bad = 0.0f;
-  for (int j = threadIdx.x; j < top; j += blockDim.x) {
-    const long long id = load_index(ids_in, bits, base + j);
-    float t = load_float(logits, dtype, base + j) * inv_t;
-    const bool listed = id >= 0 && t != -INFINITY;
-    if (listed && (id >= vocab || !(t < INFINITY))) bad = 1.0f;
-    s_id[j] = listed ? static_cast<int32_t>(id < vocab ? id : vocab) : head::kNoLabel;
-    if (!listed) t = -INFINITY;
-    s_t[j] = t;
-    mx = fmaxf(mx, t);
-    if (listed) any = 1.0f;
-  }
-  mx = block_reduce(mx, true, buf);
-  any = block_reduce(any, true, buf);
-  bad = block_reduce(bad, true, buf);
-  float sum = 0.0f;
-  for (int j = threadIdx.x; j < top; j += blockDim.x) sum += any != 0.0f ? expf(s_t[j] - mx) : 0.0f;
-  sum = block_reduce(sum, false, buf);  // also orders the writes of s_id before the ranks below
-  const float log_sum = logf(sum), inv = any != 0.0f ? 1.0f / sum : 0.0f;
-  float ent = 0.0f;
-  for (int j = threadIdx.x; j < top; j += blockDim.x) {
-    const int32_t id = s_id[j];
-    int place = 0;
-    for (int i = 0; i < top; ++i) {
-      const int32_t o = s_id[i];
-      place += (o < id || (o == id && i < j)) ? 1 : 0;
+  float mx = -INFINITY;
+  int any = 0, bad = 0;
+  for (int j = threadIdx.x; j < n; j += blockDim.x) {
+    uint32_t id32 = head::kNoLabel;
+    if (j < top) {
+      const long long id = load_index(ids_in, bits, base + j);
+      float t = load_float(logits, dtype, base + j) * inv_t;
+      const bool listed = id >= 0 && t != -INFINITY;
+      if (listed) {
+        any = 1;
+        if (id >= vocab || !(t < INFINITY)) bad = 1;
+        if (id < vocab) id32 = static_cast<uint32_t>(id);
+        mx = fmaxf(mx, t);
+      } else {
+        t = -INFINITY;
+      }
+      s_t[j] = t;
     }
-    const float d = s_t[j] - mx;
+    key[j] = (static_cast<uint64_t>(id32) << 32) | static_cast<uint32_t>(j);
+  }
+  any = __syncthreads_or(any);
+  bad = __syncthreads_or(bad);
+  mx = block_reduce(mx, true, buf);
+  float sum = 0.0f;
+  for (int j = threadIdx.x; j < top; j += blockDim.x) sum += any ? expf(s_t[j] - mx) : 0.0f;
+  sum = block_reduce(sum, false, buf);
+  for (int size = 2; size <= n; size <<= 1) {
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      for (int i = threadIdx.x; i < n / 2; i += blockDim.x) {
+        const int lo = ((i & ~(stride - 1)) << 1) | (i & (stride - 1)), hi = lo + stride;
+        const uint64_t a = key[lo], b = key[hi];
+        if ((a > b) == ((lo & size) == 0)) {
+          key[lo] = b;
+          key[hi] = a;
+        }
+      }
+      __syncthreads();
+    }
+  }
+  const float log_sum = logf(sum), inv = any ? 1.0f / sum : 0.0f;
+  float ent = 0.0f;
+  for (int place = threadIdx.x; place < top; place += blockDim.x) {
+    const uint64_t k = key[place];
+    const int32_t id = static_cast<int32_t>(k >> 32);
+    const float d = s_t[static_cast<uint32_t>(k)] - mx;
     const float p = id != head::kNoLabel ? expf(d) * inv : 0.0f;
-    ids[base + place] = id < vocab ? id : head::kNoLabel;
+    ids[base + place] = id;
     probs[base + place] = p;
     if (p > 0.0f) ent += p * (d - log_sum);
   }
   ent = block_reduce(ent, false, buf);
   if (threadIdx.x == 0) {
-    weight[row] = any == 0.0f ? 0.0f : (bad != 0.0f ? NAN : 1.0f);
+    weight[row] = !any ? 0.0f : (bad ? NAN : 1.0f);
     neg_entropy[row] = ent;
   }
 }
@@ -543,8 +561,9 @@ int launch(KernelFn fn, const Tiling& t, Params* p, const CUtensorMap (&maps)[4]
 
 // A small kernel that begins with griddep_wait: its launch overlaps the end of the kernel before it.
 template <typename... Args, typename... Actual>
-int launch_small(void (*fn)(Args...), unsigned grid, unsigned threads, cudaStream_t stream, Actual... args) {
+int launch_small(void (*fn)(Args...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, Actual... args) {
   cudaLaunchConfig_t cfg = {};
+  cfg.dynamicSmemBytes = smem;
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(threads);
   cfg.stream = stream;
@@ -662,8 +681,10 @@ int b200_head_loss_forward(const b200_head_desc* desc, const void* x, const void
   rc = status_words(&status);
   if (rc != B200_OK) return rc;
   if (d.kind == B200_HEAD_DISTILL) {
-    const unsigned threads = d.top <= 32 ? 32u : (d.top <= 64 ? 64u : (d.top <= 128 ? 128u : 256u));
-    rc = launch_small(teacher_kernel, static_cast<unsigned>(d.tokens), threads, s, teacher_logits, d.dtype_teacher, labels, d.index_bits, d.top, static_cast<int>(d.vocab),
+    int n = 2;
+    while (n < d.top) n *= 2;
+    const unsigned threads = static_cast<unsigned>(std::max(32, n / 2));
+    rc = launch_small(teacher_kernel, static_cast<unsigned>(d.tokens), threads, static_cast<size_t>(n) * 12u, s, teacher_logits, d.dtype_teacher, labels, d.index_bits, d.top, n, static_cast<int>(d.vocab),
                       1.0f / d.temperature, reinterpret_cast<int32_t*>(sv + pl.s_ids), reinterpret_cast<float*>(sv + pl.s_probs), reinterpret_cast<float*>(sv + pl.s_weight),
                       reinterpret_cast<float*>(ws + pl.f_entropy));
     if (rc != B200_OK) return rc;
@@ -712,7 +733,7 @@ int b200_head_loss_forward(const b200_head_desc* desc, const void* x, const void
   j.share = reinterpret_cast<float*>(sv);
   j.block_sums = reinterpret_cast<float2*>(ws + pl.f_sums);
   j.ticket = p.ticket;
-  return launch_small(join_kernel, static_cast<unsigned>(div_up(d.tokens, kJoinRows)), kJoinThreads, s, j);
+  return launch_small(join_kernel, static_cast<unsigned>(div_up(d.tokens, kJoinRows)), kJoinThreads, 0u, s, j);
 }
 
 int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const void* w, const void* labels, const float* lse, const void* saved,
@@ -742,7 +763,7 @@ int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const voi
   const float* weight = distill ? reinterpret_cast<const float*>(sv + pl.s_weight) : nullptr;
   const float* share = reinterpret_cast<const float*>(sv);
   if (per_row) {
-    rc = launch_small(factor_kernel, 1u, 1024u, s, grad_loss, row_scale, labels, d.index_bits, d.ignore_index, static_cast<int>(d.vocab), weight,
+    rc = launch_small(factor_kernel, 1u, 1024u, 0u, s, grad_loss, row_scale, labels, d.index_bits, d.ignore_index, static_cast<int>(d.vocab), weight,
                       static_cast<int>(d.tokens), coef_top, coef, unscale);
     if (rc != B200_OK) return rc;
   }
@@ -837,9 +858,9 @@ int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const voi
     const size_t n4 = static_cast<size_t>(d.tokens) * static_cast<size_t>(d.hidden) / 4;
     const unsigned blocks = static_cast<unsigned>(std::min<size_t>((n4 + 255) / 256, kSms * 8));
     if (d.dtype == B200_F16) {
-      return launch_small(sum_parts_kernel<__half>, blocks, 256u, s, parts, pl.splits, n4, static_cast<__half*>(grad_x));
+      return launch_small(sum_parts_kernel<__half>, blocks, 256u, 0u, s, parts, pl.splits, n4, static_cast<__half*>(grad_x));
     }
-    return launch_small(sum_parts_kernel<__nv_bfloat16>, blocks, 256u, s, parts, pl.splits, n4, static_cast<__nv_bfloat16*>(grad_x));
+    return launch_small(sum_parts_kernel<__nv_bfloat16>, blocks, 256u, 0u, s, parts, pl.splits, n4, static_cast<__nv_bfloat16*>(grad_x));
   }
   return B200_OK;
 }
