@@ -750,8 +750,8 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
   // 512 x 8192 x 8192 21.7 / 23.6 / 18.3, 22.5; 256 x 8192 x 8192 14.2 / 15.5 / 17.0, 13.6.
   //
   // Up to 128 rows the product streams B from DRAM: one CTA per tile, and the width whose rounds move the
-  // fewest columns per SM (16 x 8192 x 8192: 9.6 us with 128 tiles of 64 columns, 12.5 with 64 of 128, each
-  // cut in two along K).
+  // fewest columns per SM (16 x 8192 x 8192: 12.0 us with 128 tiles of 64 columns, 12.5 with 64 of 128, each
+  // cut in two along K; an MMA takes as long for 64 columns as for 100 or so, which keeps the two so close).
   int mx4_bn = 0, mx4_cg = 0;
   if (mx == gemm::kMx4 && d.tile_n == 0 && d.M <= gemm::kBM && cg != 2) {
     cg = 1;

@@ -140,7 +140,7 @@ typedef struct b200_gemm_desc {
   int32_t tile_m;    /* CTA tile rows: 128 (one CTA) or 256 (CTA pair); 0 = choose.  With 0 and
                       * M <= 64 a stage holds only 32 or 64 rows of A (more ring slots for B);
                       * 128 asks for full A stages                                              */
-  int32_t tile_n;    /* CTA tile columns: 64, 128 or 256; 0 = choose                            */
+  int32_t tile_n;    /* CTA tile columns: 64, 128 or 256 (fp4 pairs also 192); 0 = choose       */
   int32_t tile_k;    /* elements per pipeline stage along K; 0 = 128 bytes' worth               */
   int32_t stages;    /* shared-memory ring depth (<= 16); 0 = as many as fit, up to 8; with short
                       * A stages as many as keep 112 KB of B tiles on request (7 of 16 KB)      */
@@ -286,7 +286,7 @@ int b200_add_relu_f32(const float* a, const float* b, float* out, size_t n, void
 
 /* ---- block-scaled fp8 and fp4 (dtype_ab = B200_MXE4M3 | B200_MXE5M2 | B200_MXE2M1) --------
  * C = (A * 2^(sa-127)) . (B * 2^(sb-127))^T with sa[M][K/32], sb[N][K/32] bytes.  K % 32 == 0;
- * row-major B; tile_n 128 or 256.  The kernel streams the scales in blocks of
+ * row-major B; tile_n 128 or 256 (fp4: also 64 on one CTA and 192 on a pair; fp4 has no split_k).  The kernel streams the scales in blocks of
  * [128 rows][4 K blocks]; b200_pack_mx_scales turns row-major scales (device memory,
  * [rows][K/32] bytes) into that order (device memory of b200_mx_scales_bytes bytes, 16-byte
  * aligned).  b200_gemm_plan_set_mx_scales attaches the packed scales of A and B to a plan;
