@@ -489,11 +489,10 @@ uint32_t idesc(int dtype, const Tiling& t, bool a_mn, bool b_mn) {
 // and the kernels' shared-memory limit there.
 constexpr int kMaxDevices = 64;
 struct DeviceState {
-  std::once_flag once;
-  int rc = B200_OK;
-  char error[256] = {};
+  std::atomic<bool> ready{false};  // set once everything below is known; a failed attempt is made again by the next call
   uint32_t* status = nullptr;
 };
+std::mutex g_devices_mu;
 DeviceState g_devices[kMaxDevices];
 
 int init_device(int dev, DeviceState* st) {
@@ -518,11 +517,14 @@ int current_device(DeviceState** out) {
   B200_CUDA_OK(cudaGetDevice(&dev));
   B200_REQUIRE(dev >= 0 && dev < kMaxDevices, "head_loss: device index %d", dev);
   DeviceState& st = g_devices[dev];
-  std::call_once(st.once, [&] {
-    st.rc = init_device(dev, &st);
-    if (st.rc != B200_OK) std::snprintf(st.error, sizeof(st.error), "%s", b200_last_error());
-  });
-  if (st.rc != B200_OK) return b200::fail(st.rc, "%s", st.error);
+  if (!st.ready.load(std::memory_order_acquire)) {
+    std::lock_guard<std::mutex> lock(g_devices_mu);
+    if (!st.ready.load(std::memory_order_relaxed)) {
+      const int rc = init_device(dev, &st);
+      if (rc != B200_OK) return rc;
+      st.ready.store(true, std::memory_order_release);
+    }
+  }
   *out = &st;
   return B200_OK;
 }

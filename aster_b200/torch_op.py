@@ -27,6 +27,7 @@ before each product.  Each of the three has a ``..._direct`` twin without the di
 
 from __future__ import annotations
 
+import ctypes as C
 import threading
 from typing import Optional
 
@@ -146,16 +147,28 @@ _mx_lock = threading.Lock()
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
+_prepared_devices: set = set()
+
+
+def _prepare(device: torch.device) -> None:
+    """What the library asks of a device once: not possible while a stream is being captured."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the first call on a device sets the library up there: make it before the stream capture")
+    nat.init_current()
+    nat.call("b200_head_loss_status", (C.c_uint32 * 4)())  # kernel attributes, address of the status words
+    _ready_devices.add(device.index)
+    _prepared_devices.add(device.index)
+
+
 def _call(device: torch.device, fn, *args) -> None:
     """``fn(*args, stream)`` with torch's current stream of ``device``, with ``device`` current (the C ABI
     works on the current device, like torch)."""
-    if device.index in _ready_devices and _current_device() == device.index:
+    if device.index in _prepared_devices and _current_device() == device.index:
         status = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            if device.index not in _ready_devices:
-                nat.init_current()
-                _ready_devices.add(device.index)
+            if device.index not in _prepared_devices:
+                _prepare(device)
             status = fn(*args, _raw_stream(device))
     if status != nat.OK:
         nat.check(status)
@@ -228,7 +241,7 @@ def gemm_mx_nt_direct(a: torch.Tensor, scales_a: torch.Tensor, b: torch.Tensor, 
                       relu: bool = False, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """``epilogue(A . B^T)`` of two block-scaled fp4 operands as :func:`quantize_mx_direct` returns
     them: ``a`` ``[M, K/2]``, ``b`` ``[N, K/2]``, optional float32 ``bias`` ``[N]`` and ReLU, fp32
-    accumulation, ``[M, N]`` out.  The first call of a shape allocates: make it before a stream capture."""
+    accumulation, ``[M, N]`` out.  The first call of a shape allocates: inside a stream capture it is refused."""
     _check_mx_operand("a", a, scales_a)
     _check_mx_operand("b", b, scales_b)
     if a.device != b.device or a.shape[1] != b.shape[1]:
@@ -253,6 +266,8 @@ def _gemm_mx(a, scales_a, b, scales_b, bias, relu, out, stream) -> int:
         key = (a.device.index, M, N, K, "mxe2m1", _OUT_DTYPES[out.dtype], _EPILOGUES[(bias is not None, relu)])
         hit = _plans.get(key)
         if hit is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"the first product of a shape ({M} x {N} x {K}) allocates: make it before the stream capture")
             hit = _plans[key] = (GemmPlan(*key[1:6], epilogue=key[6]), None)
         handle = hit[0].handle
         status = lib.b200_gemm_plan_set_mx_scales(handle, scales_a.data_ptr(), scales_b.data_ptr())
@@ -294,6 +309,8 @@ def _(a, scales_a, b, scales_b, bias=None, relu=False, out_dtype=torch.float32):
 
 
 def clear_plan_cache() -> None:
+    """Destroy the plans of all shapes seen so far; not while a captured graph that holds one of their
+    products may still be replayed (a launch reports into its plan's status words)."""
     for plan, _ in _plans.values():
         plan.destroy()
     _plans.clear()

@@ -314,6 +314,49 @@ class TestProductOnGpu:
             with pytest.raises(RuntimeError):
                 top.gemm_mx_nt_direct(*args)
 
+    def test_first_call_inside_a_capture_is_refused(self, gpu):
+        q, s = top.quantize_mx_direct(torch.randn(23, 96, device="cuda"))
+        with pytest.raises(RuntimeError, match="before the stream capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                top.gemm_mx_nt_direct(q, s, q, s)
+        want = top.gemm_mx_nt_direct(q, s, q, s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c = top.gemm_mx_nt_direct(q, s, q, s)
+        graph.replay()
+        assert torch.equal(c, want)
+
+    def test_first_use_of_the_library_inside_a_capture_is_refused(self, gpu):
+        """In a process of its own: refused, and everything works afterwards."""
+        import subprocess
+        import sys
+
+        code = """
+import torch
+import aster_b200.torch_op as top, aster_b200.head_loss as hl
+x = torch.randn(16, 64, device="cuda").bfloat16()
+t = torch.zeros(16, dtype=torch.long, device="cuda")
+for call in (lambda: top.quantize_mx_direct(x), lambda: hl.linear_cross_entropy(x, x, t)):
+    try:
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            call()
+        raise SystemExit("not refused")
+    except RuntimeError as e:
+        assert "before the stream capture" in str(e), e
+hl.linear_cross_entropy(x, x, t)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    loss, (q, s) = hl.linear_cross_entropy(x, x, t), top.quantize_mx_direct(x)
+graph.replay()
+assert torch.equal(loss, hl.linear_cross_entropy(x, x, t)) and torch.equal(q, top.quantize_mx_direct(x)[0])
+print("ok")
+"""
+        import os
+
+        root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+        out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root, timeout=300)
+        assert out.returncode == 0 and out.stdout.strip().endswith("ok"), out.stderr[-2000:]
+
     def test_from_other_threads(self, gpu):
         """A thread whose first CUDA call is the product, and several that share one plan."""
         import threading
