@@ -340,8 +340,9 @@ struct Tiling {
 
 int ring(Tiling* t) {
   const int room = kMaxSmem - head::kBarrierBytes - 1024 - t->warps * head::kTurnBytes - head::overrun_bytes(t->bn, t->cg, t->am);
-  // With few rows the product streams w from DRAM, which is fastest with about 112 KB of it on request per SM.
-  const int cap = t->am < 128 ? std::max(4, 112 * 1024 / (t->bn * head::kRowBytes)) : 8;
+  // With few rows the product streams w from DRAM, and 140 KB of it on request per SM are enough (8 x 4096 x 32768
+  // forward: 61 / 55 / 54 / 53 / 53 us with 2 / 3 / 4 / 5 / 6 stages of 28 KB).
+  const int cap = t->am < 128 ? std::min(head::kMaxStages, std::max(4, 140 * 1024 / (t->bn * head::kRowBytes))) : 8;
   t->stages = std::min(cap, room / head::stage_bytes(t->bn, t->cg, t->am));
   t->smem = head::smem_bytes(t->bn, t->stages, t->cg, t->am, t->warps);
   // One CTA per SM: each takes all of TMEM.

@@ -124,7 +124,8 @@ def teacher(T, V, top, g, dtype=torch.float32, duplicates=False):
     return ids, logits
 
 
-SHAPES = [(1, 8, 1), (1, 64, 50), (7, 64, 257), (33, 128, 1000), (65, 200, 130), (128, 256, 512), (130, 72, 4097), (257, 264, 3001), (300, 520, 2048), (600, 1032, 5003)]
+SHAPES = [(1, 8, 1), (1, 64, 50), (7, 64, 257), (33, 128, 1000), (65, 200, 130), (128, 256, 512), (130, 72, 4097), (257, 264, 3001), (300, 520, 2048), (600, 1032, 5003),
+          (3, 1040, 261), (20, 2056, 700), (50, 1200, 90)]
 
 
 class TestOnHost:
