@@ -316,6 +316,7 @@ struct b200_gemm_plan {
   // Tail split (see gemm::Params): decided from the tile count and the persistent grid.
   int units_cap = kDefaultSms;  // CTAs (pairs) the persistent grid may use
   int tail_tiles = 0, tail_parts = 0, tail_kb0 = 0, tail_kb = 0;
+  int parts_choice = 0;        // parts per tile that the plan's cost model asked for (1: none); 0 = by the rule above plan_tail_split
   int64_t tail_ws_bytes = 0;   // flags + partial tiles; 0 = tail split not useful for this plan
   int64_t tail_flag_bytes = 0;
   // The parts of every tile are the CTAs of one cluster and exchange their partial sums through
@@ -357,7 +358,7 @@ void plan_tail_split(b200_gemm_plan* plan) {
   plan->tail_tiles = plan->tail_parts = plan->tail_kb0 = plan->tail_kb = 0;
   plan->tail_ws_bytes = plan->tail_flag_bytes = 0;
   plan->cluster_exchange = false;
-  if (plan->split_k > 1 || (plan->desc.reserved[1] & 1) != 0) return;  // reserved[1] bit 0: caller opted out
+  if (plan->split_k > 1 || plan->parts_choice == 1 || (plan->desc.reserved[1] & 1) != 0) return;  // reserved[1] bit 0: caller opted out
   if (plan->desc.dtype_ab == B200_I8) return;  // partial tiles are exchanged as fp32; s32 sums stay whole
   const int units = plan->units_cap;
   const int tiles = plan->m_blocks * plan->n_blocks;
@@ -370,9 +371,10 @@ void plan_tail_split(b200_gemm_plan* plan) {
   // split that saves fewer than ~12 K blocks per unit makes the launch longer (512^3: 8 K blocks,
   // 9.3 -> 6 us per launch without the split).
   // (4-bit: twice that -- an SM alone streams a short tile faster than two exchange it.)
-  const int min_kb_per_part = plan->mx == gemm::kMx4 ? 24 : 12;
+  const int min_kb_per_part = plan->parts_choice > 1 ? 1 : (plan->mx == gemm::kMx4 ? 24 : 12);
   int parts = 0;
   for (int cand = 8; cand >= 2; cand /= 2) {
+    if (plan->parts_choice > 0 && cand != plan->parts_choice) continue;
     if (cand > units / tail || plan->bn / cand < 32 || plan->bn % (32 * cand) != 0 || plan->num_kb / cand < min_kb_per_part) continue;
     const int per = (plan->num_kb + cand - 1) / cand;
     if ((plan->num_kb + per - 1) / per != cand) continue;
@@ -749,13 +751,30 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
   // columns on pairs, 128 on one CTA): 8192^3 232 / 188 / 224, 279; 4096^3 40.6 / 33.7 / 42.0, 42.4;
   // 512 x 8192 x 8192 21.7 / 23.6 / 18.3, 22.5; 256 x 8192 x 8192 14.2 / 15.5 / 17.0, 13.6.
   //
-  // Up to 128 rows the product streams B from DRAM: one CTA per tile, and the width whose rounds move the
-  // fewest columns per SM (16 x 8192 x 8192: 12.0 us with 128 tiles of 64 columns, 12.5 with 64 of 128, each
-  // cut in two along K; an MMA takes as long for 64 columns as for 100 or so, which keeps the two so close).
+  // Up to 128 rows the product streams B from DRAM (6.2 TB/s), but its MMAs come one after the other: a stage of
+  // a 64-column tile takes 0.235 us and one of a 128-column tile 0.28, whatever the rows.  So a tile's K is cut
+  // between the CTAs of a cluster where that saves more than the 2.5 us of their exchange, as long as all of
+  // them run at once (us, uncut or in two -> as chosen here: 1 x 1024 x 8192 10.6 -> 8.2,
+  // 16 x 8192 x 16384 19.5 -> 17.6, 4 x 4096 x 16384 14.0 -> 13.5; 16 x 8192 x 8192 takes 12.0 with 128 uncut
+  // tiles of 64 columns, 12.5 with 64 of 128 cut in two).
   int mx4_bn = 0, mx4_cg = 0;
   if (mx == gemm::kMx4 && d.tile_n == 0 && d.M <= gemm::kBM && cg != 2) {
     cg = 1;
-    mx4_bn = ceil_div(ceil_div(d.N, 64), kDefaultSms) * 64 < ceil_div(ceil_div(d.N, 128), kDefaultSms) * 128 ? 64 : 128;
+    const double dram_us = static_cast<double>(d.N) * static_cast<double>(d.K) * (17.0 / 32.0) / 6.2e6;
+    double best = 0.0;
+    for (int parts : {1, 2, 4}) {
+      for (int bn : {128, 64}) {
+        const int64_t tiles = ceil_div(d.N, bn);
+        if (bn / parts < 32 || k_blocks < 2 * parts || (parts > 1 && tiles * parts > kDefaultSms)) continue;
+        const double compute_us = static_cast<double>((tiles * parts + kDefaultSms - 1) / kDefaultSms) * ceil_div(k_blocks, parts) * (bn == 64 ? 0.235 : 0.28);
+        const double us = std::max(compute_us, dram_us) + (parts > 1 ? 2.5 : 0.0);
+        if (mx4_bn == 0 || us < best - 1e-9) {
+          mx4_bn = bn;
+          plan->parts_choice = parts;
+          best = us;
+        }
+      }
+    }
   } else if (mx == gemm::kMx4 && d.tile_n == 0) {
     static const struct {
       int cg, bn;
