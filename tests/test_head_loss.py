@@ -519,6 +519,28 @@ class TestDistillation:
         x.requires_grad_(), w.requires_grad_()
         ref.check_grads(*torch.autograd.grad(hl.linear_distillation(x, w, logits, ids, temperature=2.0, grad_bytes=300 * 2 * 512), (x, w)))
 
+    @pytest.mark.parametrize("operand", ["x", "w"])
+    def test_against_differences(self, gpu, operand):
+        x, w, g = make(40, 64, 300, F16, 28)
+        ids, logits = teacher(40, 300, 12, g)
+        loss64 = lambda x, w: distill_reference(x, w, logits, ids, 1.5, reduction="sum")
+        base = x if operand == "x" else w
+        step = 2.0 ** -4 * torch.randn(base.shape, device="cuda", generator=g) * base.float().std()
+        a, b = (base.float() - step).half(), (base.float() + step).half()
+        mid = ((a.double() + b.double()) / 2).half()
+        at = lambda v: (v, w) if operand == "x" else (x, v)
+        difference = float(loss64(*at(b)).loss - loss64(*at(a)).loss)
+        ref = loss64(*at(mid))
+        mid.requires_grad_()
+        got, = torch.autograd.grad(hl.linear_distillation(*at(mid), logits, ids, temperature=1.5, reduction="sum"), mid)
+        delta = b.double() - a.double()
+        want, spread = (ref.dx, ref.g.abs() @ ref.w.abs()) if operand == "x" else (ref.dw, ref.g.T.abs() @ ref.x.abs())
+        # what the difference quotient itself misses (and the rounding of the midpoint), from the 64-bit gradient
+        quotient = abs(difference - float((want * delta).sum()))
+        tol = quotient + 2.0 ** -10 * float((spread * delta.abs()).sum())
+        assert abs(float((got.double() * delta).sum()) - difference) <= tol
+        assert quotient < 0.1 * abs(difference)
+
     def test_one_certain_entry_is_cross_entropy(self, gpu):
         x, w, g = make(60, 64, 500, BF16, 23)
         t = targets(60, 500, g)
