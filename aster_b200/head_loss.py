@@ -38,6 +38,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     """Two dimensions, the last one contiguous, rows a multiple of 16 bytes apart and aligned (else a copy)."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
     if t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1])):
         t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
@@ -98,6 +100,17 @@ class _Head:
         if kind == nat.HEAD_DISTILL:
             d.top, d.dtype_teacher = labels.shape[-1], nat.F32 if teacher is None else _TEACHER_DTYPES[teacher.dtype]
         self.per_row = reduction == "none"
+
+    def without_tensors(self) -> "_Head":
+        """The description alone, for the time until the backward pass brings the tensors again."""
+        h = _Head.__new__(_Head)
+        h.desc, h.per_row = self.desc, self.per_row
+        return h
+
+    def with_tensors(self, x, w, labels) -> "_Head":
+        h = self.without_tensors()  # its own object: a graph may be walked from several threads
+        h.x, h.w, h.labels, h.teacher = _rows(x), _rows(w), labels, None
+        return h
 
     def forward(self):
         dev, tokens = self.x.device, self.x.shape[0]
@@ -185,18 +198,15 @@ class _HeadLoss(torch.autograd.Function):
         loss, lse, saved = head.forward()
         # the tensors come back through save_for_backward: it notices a change in place before the backward pass
         ctx.save_for_backward(x, w, head.labels, lse, saved)
-        ctx.desc_args, ctx.shape = head.desc, x.shape
-        ctx.per_row = head.per_row
+        ctx.head, ctx.shape = head.without_tensors(), x.shape
         return loss.view(shape) if head.per_row else loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         x, w, labels, lse, saved = ctx.saved_tensors
-        head = _Head.__new__(_Head)
-        head.x, head.w, head.labels, head.teacher, head.desc, head.per_row = _rows(x), _rows(w), labels, None, ctx.desc_args, ctx.per_row
-        dx, dw = head.backward(grad, lse, saved, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
-        return None if dx is None else dx.view(ctx.shape), dw, None, None
+        dx, dw = ctx.head.with_tensors(x, w, labels).backward(grad, lse, saved, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return dx if dx is None or dx.dim() == len(ctx.shape) else dx.view(ctx.shape), dw, None, None
 
 
 def _apply(x: torch.Tensor, w: torch.Tensor, head: _Head, shape) -> torch.Tensor:
