@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(1024) factor_kernel(const float* __restrict__ 
   if (threadIdx.x == 0) *unscale = mx / top;
 }
 
-// dX = sum of its fp32 parts, in their order, rounded once.  n4 = elements / 4.
+// A gradient as the sum of its fp32 parts, in their order, rounded once.  n4 = elements / 4.
 template <typename T16>
 __global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ parts, int splits, size_t n4, T16* __restrict__ out) {
   sm100::griddep_wait();
@@ -379,12 +379,13 @@ struct Plan {
   int64_t n_blocks;       // tiles along the vocabulary, forward
   int64_t range, ranges;  // columns of G at a time
   int64_t g_ld;
-  int splits, kb_per_split;
+  int splits, kb_per_split;      // of dX's K, the range
+  int w_splits, w_kb_per_split;  // of dW's K, the tokens
   bool direct;            // dX is written by the product itself
   // byte offsets
   size_t f_part, f_part_z, f_label_z, f_entropy, f_sums, f_ticket, f_bytes;
   size_t s_weight, s_probs, s_ids, s_bytes;
-  size_t b_g, b_coef, b_unscale, b_parts, b_bytes;
+  size_t b_g, b_coef, b_unscale, b_parts, b_w_parts, b_bytes;
 };
 
 int make_plan(const b200_head_desc& d, Plan* p) {
@@ -456,11 +457,19 @@ int make_plan(const b200_head_desc& d, Plan* p) {
   p->kb_per_split = static_cast<int>(div_up(x_kb, parts));
   p->splits = static_cast<int>(div_up(x_kb, p->kb_per_split));
   p->direct = p->splits == 1 && p->ranges == 1;
+  // dW likewise where one of its tiles is more than an SM's share of all the work (a small vocabulary or hidden axis
+  // and many tokens: 65536 x 256 x 4000 backward 1111 -> 720 us, 8192 x 256 x 4000 98 -> 86) and the fp32 parts stay
+  // below 256 MiB; with shorter tiles the parts only cost (8192 x 1024 x 4096: 152 -> 162).
+  const int64_t part_bytes = p->range * d.hidden * 4;
+  const int64_t w_parts = w_kb > share ? std::min<int64_t>({16, div_up(w_kb, want), std::max<int64_t>(1, kGradBytes / part_bytes)}) : 1;
+  p->w_kb_per_split = static_cast<int>(div_up(w_kb, w_parts));
+  p->w_splits = static_cast<int>(div_up(w_kb, p->w_kb_per_split));
   at = 0;
   p->b_g = take(T * static_cast<size_t>(p->g_ld) * 2);
   p->b_coef = take(T * sizeof(float));
   p->b_unscale = take(sizeof(float));
   p->b_parts = take(p->direct ? 0 : static_cast<size_t>(p->splits) * T * static_cast<size_t>(d.hidden) * sizeof(float));
+  p->b_w_parts = take(p->w_splits > 1 ? static_cast<size_t>(p->w_splits) * static_cast<size_t>(part_bytes) : 0);
   p->b_bytes = at;
   return B200_OK;
 }
@@ -579,6 +588,13 @@ int launch_small(void (*fn)(Args...), unsigned grid, unsigned threads, size_t sm
   b200::count_launch();
   B200_CUDA_OK(cudaGetLastError());
   return B200_OK;
+}
+
+int launch_sum_parts(int dtype, const float* parts, int splits, size_t n, void* out, cudaStream_t stream) {
+  const size_t n4 = n / 4;
+  const unsigned blocks = static_cast<unsigned>(std::min<size_t>((n4 + 255) / 256, kSms * 8));
+  if (dtype == B200_F16) return launch_small(sum_parts_kernel<__half>, blocks, 256u, 0u, stream, parts, splits, n4, static_cast<__half*>(out));
+  return launch_small(sum_parts_kernel<__nv_bfloat16>, blocks, 256u, 0u, stream, parts, splits, n4, static_cast<__nv_bfloat16*>(out));
 }
 
 // z = x . w^T over the columns [col0, col0 + cols).
@@ -840,30 +856,32 @@ int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const voi
       maps[2 * q.num_probs + 1] = x_rows;
       dw.M = static_cast<int>(cols);
       dw.N = static_cast<int>(d.hidden);
-      dw.num_kb = dw.kb_per_split = static_cast<int>(div_up(d.tokens, head::kStageK));
-      dw.splits = 1;
+      dw.num_kb = static_cast<int>(div_up(d.tokens, head::kStageK));
+      dw.kb_per_split = pl.w_kb_per_split;
+      dw.splits = pl.w_splits;
       dw.m_blocks = static_cast<int>(div_up(cols, 128 * pl.prod.cg));
       dw.n_blocks = static_cast<int>(div_up(d.hidden, pl.prod.bn));
       dw.raster_group = raster(dw.m_blocks, 128 * pl.prod.cg, d.tokens);
       dw.a_mn = dw.b_mn = 1;
       dw.idesc = idesc(d.dtype, pl.prod, true, true);
       dw.ld = d.hidden;
-      dw.out16 = static_cast<uint8_t*>(grad_w) + static_cast<size_t>(col0) * d.hidden * 2;
+      dw.out16 = pl.w_splits > 1 ? nullptr : static_cast<uint8_t*>(grad_w) + static_cast<size_t>(col0) * d.hidden * 2;
+      dw.partial = reinterpret_cast<float*>(ws + pl.b_w_parts);
       rc = set_items(&dw);
       if (rc != B200_OK) return rc;
       ++q.num_probs;
     }
-    if (q.num_probs == 2) q.extra_rounds = std::max(1, q.prob[0].kb_per_split / q.prob[1].num_kb);
+    if (q.num_probs == 2) q.extra_rounds = std::max(1, q.prob[0].kb_per_split / q.prob[1].kb_per_split);
     rc = launch(kernel_for<head::kProduct>(pl.prod.cg, d.dtype, pl.prod.warps), pl.prod, &q, maps, s);
     if (rc != B200_OK) return rc;
+    if (grad_w != nullptr && pl.w_splits > 1) {
+      rc = launch_sum_parts(d.dtype, reinterpret_cast<const float*>(ws + pl.b_w_parts), pl.w_splits, static_cast<size_t>(cols) * static_cast<size_t>(d.hidden),
+                            static_cast<uint8_t*>(grad_w) + static_cast<size_t>(col0) * d.hidden * 2, s);
+      if (rc != B200_OK) return rc;
+    }
   }
   if (grad_x != nullptr && !pl.direct) {
-    const size_t n4 = static_cast<size_t>(d.tokens) * static_cast<size_t>(d.hidden) / 4;
-    const unsigned blocks = static_cast<unsigned>(std::min<size_t>((n4 + 255) / 256, kSms * 8));
-    if (d.dtype == B200_F16) {
-      return launch_small(sum_parts_kernel<__half>, blocks, 256u, 0u, s, parts, pl.splits, n4, static_cast<__half*>(grad_x));
-    }
-    return launch_small(sum_parts_kernel<__nv_bfloat16>, blocks, 256u, 0u, s, parts, pl.splits, n4, static_cast<__nv_bfloat16*>(grad_x));
+    return launch_sum_parts(d.dtype, parts, pl.splits, static_cast<size_t>(d.tokens) * static_cast<size_t>(d.hidden), grad_x, s);
   }
   return B200_OK;
 }
