@@ -94,6 +94,7 @@ class _Head:
 
     def __init__(self, x, w, labels, reduction, *, kind, ignore_index=0, label_smoothing=0.0, temperature=1.0, teacher=None, grad_bytes=0):
         self.x, self.w, self.labels, self.teacher = _rows(x), _rows(w), labels.contiguous(), teacher
+        self.device, self.shapes = x.device, (self.x.shape, self.w.shape, self.labels.shape)
         self.desc = d = _desc(self.x, self.w, labels, reduction)
         d.kind, d.ignore_index, d.label_smoothing, d.temperature = kind, ignore_index, label_smoothing, temperature
         d.grad_bytes = grad_bytes
@@ -104,12 +105,24 @@ class _Head:
     def without_tensors(self) -> "_Head":
         """The description alone, for the time until the backward pass brings the tensors again."""
         h = _Head.__new__(_Head)
-        h.desc, h.per_row = self.desc, self.per_row
+        h.desc, h.per_row, h.device, h.shapes = self.desc, self.per_row, self.device, self.shapes
         return h
 
     def with_tensors(self, x, w, labels) -> "_Head":
+        """The description with the forward pass's tensors, as they come back from autograd.  Hooks on saved
+        tensors may have laid them out anew (an offloaded slice returns contiguous): the strides are theirs."""
         h = self.without_tensors()  # its own object: a graph may be walked from several threads
-        h.x, h.w, h.labels, h.teacher = _rows(x), _rows(w), labels, None
+        h.x, h.w, h.labels, h.teacher = _rows(x), _rows(w), labels.contiguous(), None
+        x, w, labels = h.x, h.w, h.labels
+        d = self.desc
+        if (x.shape, w.shape, labels.shape) != self.shapes or _DTYPES.get(x.dtype) != d.dtype or w.dtype != x.dtype or _INDEX_BITS.get(labels.dtype) != d.index_bits:
+            raise RuntimeError("the saved tensors came back with another shape or dtype than the forward pass had")
+        if not x.device == w.device == labels.device == self.device:
+            raise RuntimeError(f"the saved tensors came back on {x.device}, {w.device} and {labels.device}, not on {self.device}")
+        strides = x.stride(0) if d.tokens > 1 else d.hidden, w.stride(0) if d.vocab > 1 else d.hidden
+        if strides != (d.x_stride, d.w_stride):
+            h.desc = nat.HeadDesc.from_buffer_copy(d)
+            h.desc.x_stride, h.desc.w_stride = strides
         return h
 
     def forward(self):
@@ -135,7 +148,11 @@ class _Head:
         dw = torch.empty(self.w.shape, dtype=self.w.dtype, device=dev) if want_w else None
         if grad.dtype != torch.float32 or not grad.is_contiguous():
             grad = grad.to(torch.float32).contiguous()
-        need = _sizes_of(bytes(self.desc)).backward_workspace
+        sizes = _sizes_of(bytes(self.desc))
+        need = sizes.backward_workspace
+        for what, t, dtype, n in (("grad", grad, torch.float32, tokens if self.per_row else 1), ("lse", lse, torch.float32, tokens), ("saved", saved, torch.uint8, sizes.saved)):
+            if t.dtype != dtype or t.device != dev or t.numel() != n or not t.is_contiguous():
+                raise RuntimeError(f"{what} must be {n} contiguous {dtype} on {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
         ws = self.x.new_empty(need, dtype=torch.uint8)
         _call(dev, nat.lib().b200_head_loss_backward, C.byref(self.desc), self.x.data_ptr(), self.w.data_ptr(), self.labels.data_ptr(), lse.data_ptr(),
               saved.data_ptr(), grad.data_ptr(), _ptr(dx), _ptr(dw), ws.data_ptr(), need)
