@@ -23,6 +23,7 @@ import weakref
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from .torch_op import _call, _raw_stream
@@ -46,6 +47,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _check(name: str, x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, reduction: str) -> None:
+    if forward_ad.unpack_dual(x).tangent is not None or forward_ad.unpack_dual(w).tangent is not None:
+        raise RuntimeError(f"aster_b200::{name} has no forward-mode derivative: x and weight must not carry a tangent")
     for what, t in (("x", x), ("weight", w), ("labels", labels)):
         if not t.is_cuda:
             raise RuntimeError(f"aster_b200::{name} needs CUDA tensors, {what} is on {t.device} (there is no CPU path)")

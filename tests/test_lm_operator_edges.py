@@ -72,3 +72,42 @@ class TestSavedTensors:
                 back(grad, x, w, t, l, s, -100, 0.0, "mean")
         with pytest.raises(RuntimeError, match="must be"):
             back(one, x, w, t, lse, saved, -100, 0.0, "none")
+
+
+class TestForwardMode:
+    """A tangent is refused, never dropped."""
+
+    @staticmethod
+    def check(x, w, t, ids, logits, dual_x, requires_grad, no_grad, dispatcher=True):
+        from torch.autograd import forward_ad
+
+        x, w = x.clone().requires_grad_(requires_grad), w.clone().requires_grad_(requires_grad)
+        ops = torch.ops.aster_b200
+        with forward_ad.dual_level(), torch.set_grad_enabled(not no_grad):
+            if dual_x:
+                x = forward_ad.make_dual(x, torch.ones_like(x))
+            else:
+                w = forward_ad.make_dual(w, torch.ones_like(w))
+            calls = [lambda: hl.linear_cross_entropy(x, w, t), lambda: hl.linear_distillation(x, w, logits, ids)]
+            if dispatcher:
+                calls += [lambda: ops.linear_cross_entropy(x, w, t), lambda: ops.linear_distillation(x, w, logits, ids)]
+            for call in calls:
+                with pytest.raises((RuntimeError, NotImplementedError), match="forward.mode"):
+                    call()
+
+    @pytest.mark.parametrize("dual_x", [True, False])
+    @pytest.mark.parametrize("requires_grad", [True, False])
+    @pytest.mark.parametrize("no_grad", [True, False])
+    def test_on_the_host(self, dual_x, requires_grad, no_grad):
+        x, w, t = strided_problem("cpu")
+        # with a graph to record, torch refuses the operators itself, but only after their forward pass
+        self.check(x, w, t, t[:, None], torch.zeros(70, 1), dual_x, requires_grad, no_grad, dispatcher=no_grad or not requires_grad)
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("dual_x", [True, False])
+    @pytest.mark.parametrize("requires_grad", [True, False])
+    @pytest.mark.parametrize("no_grad", [True, False])
+    def test_on_the_gpu(self, gpu, dual_x, requires_grad, no_grad):
+        x, w, t = strided_problem("cuda")
+        self.check(x, w, t, t[:, None], torch.zeros(70, 1, device="cuda"), dual_x, requires_grad, no_grad)
+        hl.linear_cross_entropy(x, w, t)  # without a tangent as before
