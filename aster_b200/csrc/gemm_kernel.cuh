@@ -308,6 +308,19 @@ __device__ __forceinline__ bool wait_flag(const uint32_t* flag, uint32_t want, c
   return ok != 0;
 }
 
+// ReLU of the epilogue.  A block of 4-bit elements says "not a number" with its scale, and ReLU passes
+// that on (max.NaN); the other types keep fmaxf, under which a NaN becomes 0.
+template <int MX>
+__device__ __forceinline__ float relu_of(float x) {
+  if constexpr (MX == kMx4) {
+    float y;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+    return y;
+  } else {
+    return fmaxf(x, 0.0f);
+  }
+}
+
 // Work item -> (m block, n block).  Groups of `raster_group` m-blocks are walked m-fastest so
 // that the ~148 tiles in flight share a few A row panels and B row panels in L2.
 __device__ __forceinline__ void tile_coords(const Params& p, int tile, int& m_blk, int& n_blk) {
@@ -994,7 +1007,7 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             }
             if (p.relu) {
 #pragma unroll
-              for (int j = 0; j < kCols; ++j) x[j] = fmaxf(x[j], 0.0f);
+              for (int j = 0; j < kCols; ++j) x[j] = relu_of<MX>(x[j]);
             }
             __syncwarp();  // the previous piece has been read
 #pragma unroll
@@ -1074,7 +1087,7 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
               }
               if (p.relu) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) x[j] = fmaxf(x[j], 0.0f);
+                for (int j = 0; j < 32; ++j) x[j] = relu_of<MX>(x[j]);
               }
               if (row_ok && !bringup_mode(p, 32)) {
                 store_row32<OutT>(C + static_cast<size_t>(row) * p.N + col0, x, n_vec_ok && valid == 32, valid, n_wide_ok);
@@ -1185,7 +1198,7 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         }
         if (p.relu) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) x[j] = fmaxf(x[j], 0.0f);
+          for (int j = 0; j < 32; ++j) x[j] = relu_of<MX>(x[j]);
         }
         if (row_ok && !bringup_mode(p, 32)) {
           store_row32<OutT>(C + static_cast<size_t>(row) * p.N + col0, x, n_vec_ok && valid == 32, valid, n_wide_ok);

@@ -302,7 +302,8 @@ int b200_gemm_plan_set_mx_scales(b200_gemm_plan* plan, const void* scales_a_pack
  * product streams (rows behind the last and blocks behind K get byte 127).  Per block of 32 the
  * shared exponent is floor(log2 max|x|) - 2, clamped to [-127, 127] (a block of zeros: 0), the
  * elements are x / 2^exponent rounded to nearest even and saturated at 6.  A block that holds a NaN
- * or an infinity gets scale byte 255: its 32 values read as NaN.  dtype_q = B200_MXE2M1.
+ * or an infinity gets scale byte 255: its 32 values read as NaN, and a product of them stays NaN under its
+ * ReLU (the other types' ReLU makes a NaN 0).  dtype_q = B200_MXE2M1.
  * q, scales_packed and out are 16-byte aligned; out is [rows][K] of dtype_out. */
 int b200_quantize_mx(const void* x, int32_t dtype_x, int64_t rows, int64_t K, int64_t row_stride, int32_t dtype_q,
                      void* q, void* scales_packed, void* stream);

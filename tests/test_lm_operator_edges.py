@@ -1,9 +1,13 @@
 """Calls of the language-model operators from their edges."""
 
+import numpy as np
 import pytest
 import torch
 
+import aster_b200.torch_op as top
+from aster_b200 import dtypes
 from aster_b200 import head_loss as hl
+from aster_b200.gemm import gemm
 
 BF16 = torch.bfloat16
 
@@ -111,3 +115,42 @@ class TestForwardMode:
         x, w, t = strided_problem("cuda")
         self.check(x, w, t, t[:, None], torch.zeros(70, 1, device="cuda"), dual_x, requires_grad, no_grad)
         hl.linear_cross_entropy(x, w, t)  # without a tangent as before
+
+
+def exact_operand(rows, K, rng):
+    """4-bit codes under scales of 1: products are multiples of 1/4 of at most 36, sums of a few thousand exact in fp32."""
+    q = dtypes.pack_e2m1(rng.integers(0, 16, (rows, K)).astype(np.uint8))
+    scales = np.full((rows, K // 32), 127, np.uint8)
+    return q, scales, dtypes.dequantize_mx(q, scales, "e2m1").astype(np.float64)
+
+
+@pytest.mark.gpu
+class TestNanUnderRelu:
+    @pytest.mark.parametrize("dtype_c", ["f32", "bf16"])
+    @pytest.mark.parametrize("shape", [(300, 260, 416), (300, 263, 160), (20, 264, 288), (60, 261, 416), (100, 320, 4128)])
+    @pytest.mark.parametrize("plan", [{}, {"cta_group": 1, "tile_n": 128}, {"tile_n": 64}, {"max_ctas": 2, "tail_split": True}])
+    def test_every_ending_of_the_product_keeps_it(self, gpu, dtype_c, shape, plan):
+        """Whole tiles, ragged columns, short A stages, K cut between CTAs: NaN stays, negative sums become 0."""
+        M, N, K = shape
+        rng = np.random.default_rng(M + N + K)
+        (qa, sa, a), (qb, sb, b) = exact_operand(M, K, rng), exact_operand(N, K, rng)
+        row, column = M - 2, N - 3
+        sa[row, 0] = sb[column, 1] = 255
+        bias = rng.integers(-8, 8, N).astype(np.float32)
+        got = gemm(qa, qb, dtype_ab="mxe2m1", dtype_c=dtype_c, block_scales_a=sa, block_scales_b=sb, bias=bias, relu=True, **plan)
+        got = got if dtype_c == "f32" else dtypes.bf16_bits_to_f32(got)
+        bad = np.zeros((M, N), bool)
+        bad[row], bad[:, column] = True, True
+        assert np.isnan(got[bad]).all()
+        want = np.maximum(a @ b.T + bias, 0).astype(np.float32)
+        want = want if dtype_c == "f32" else dtypes.bf16_round(want)
+        assert (want[~bad] == 0).any() and np.array_equal(got[~bad], want[~bad])
+
+    def test_from_values_to_the_layer_behind(self, gpu):
+        x = torch.randn(64, 256, device="cuda")
+        x[3, 40], x[9, 200] = float("nan"), float("inf")
+        w = top.quantize_mx_direct(torch.randn(128, 256, device="cuda"))
+        c = top.gemm_mx_nt_direct(*top.quantize_mx_direct(x), *w, relu=True)
+        bad = torch.zeros(64, dtype=torch.bool, device="cuda")
+        bad[[3, 9]] = True
+        assert torch.equal(torch.isnan(c).all(1), bad) and torch.equal(torch.isnan(c).any(1), bad) and bool((c[~bad] >= 0).all())
