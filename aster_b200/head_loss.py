@@ -186,7 +186,7 @@ def _distill_head(x, w, teacher_logits, teacher_ids, temperature, reduction, gra
     return _Head(x, w, teacher_ids, reduction, kind=nat.HEAD_DISTILL, temperature=temperature, teacher=teacher_logits, grad_bytes=grad_bytes)
 
 
-# Graphs of these functions that were made on a default stream, each with its leaves, for as long as they live.
+# Graphs of these functions and operators that were made on a default stream, each with its leaves, for as long as they live.
 # Autograd keeps one accumulation node per leaf, tied to the stream that was current when it was made, while any
 # graph refers to it.  A backward pass that is being captured cannot join the default stream, so a graph left
 # over from there would break the capture (and, from the engine's own threads, the process): such a capture is
@@ -208,13 +208,22 @@ def _note_graph(ctx, x: torch.Tensor, w: torch.Tensor) -> None:
         _default_stream_graphs[key] = (leaves, weakref.ref(ctx, lambda _: _default_stream_graphs.pop(key, None)))
 
 
+def _capturing(device: torch.device) -> bool:
+    with torch.cuda.device(device):  # of the tensors, which need not be the current one
+        return torch.cuda.is_current_stream_capturing()
+
+
+def _watch_graph(ctx, x: torch.Tensor, w: torch.Tensor) -> None:
+    if not _raw_stream(x.device):
+        _note_graph(ctx, x, w)
+    elif _capturing(x.device):
+        _refuse_capture_beside(x, w)
+
+
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, head, shape):
-        if not _raw_stream(x.device):
-            _note_graph(ctx, x, w)
-        elif torch.cuda.is_current_stream_capturing():
-            _refuse_capture_beside(x, w)
+        _watch_graph(ctx, x, w)
         loss, lse, saved = head.forward()
         # the tensors come back through save_for_backward: it notices a change in place before the backward pass
         ctx.save_for_backward(x, w, head.labels, lse, saved)
@@ -305,8 +314,14 @@ def _(grad, x, weight, target, lse, saved, ignore_index, label_smoothing, reduct
     return x.new_empty(x.shape), weight.new_empty(weight.shape)
 
 
+def _watch_operator(ctx, x: torch.Tensor, w: torch.Tensor) -> None:
+    if x.is_cuda and all(type(t) in (torch.Tensor, torch.nn.Parameter) for t in (x, w)):  # not while a compiler traces
+        _watch_graph(ctx, x, w)
+
+
 def _xent_setup(ctx, inputs, output):
     x, weight, target, ctx.ignore_index, ctx.label_smoothing, ctx.reduction = inputs
+    _watch_operator(ctx, x, weight)
     ctx.mark_non_differentiable(output[1], output[2])
     ctx.save_for_backward(x, weight, target, output[1], output[2])
 
@@ -347,6 +362,7 @@ def _(grad, x, weight, teacher_ids, lse, saved, temperature, reduction):
 
 def _distill_setup(ctx, inputs, output):
     x, weight, _, teacher_ids, ctx.temperature, ctx.reduction = inputs
+    _watch_operator(ctx, x, weight)
     ctx.mark_non_differentiable(output[1], output[2])
     ctx.save_for_backward(x, weight, teacher_ids, output[1], output[2])
 

@@ -154,3 +154,29 @@ class TestNanUnderRelu:
         bad = torch.zeros(64, dtype=torch.bool, device="cuda")
         bad[[3, 9]] = True
         assert torch.equal(torch.isnan(c).all(1), bad) and torch.equal(torch.isnan(c).any(1), bad) and bool((c[~bad] >= 0).all())
+
+
+@pytest.mark.gpu
+class TestCaptureBesideAGraph:
+    @pytest.mark.parametrize("distill", [False, True])
+    @pytest.mark.parametrize("eager", ["function", "operator"])
+    @pytest.mark.parametrize("captured", ["function", "operator"])
+    def test_every_form_is_seen_and_refused(self, gpu, distill, eager, captured):
+        x, w, t = strided_problem("cuda")
+        x, w = x.contiguous().requires_grad_(), w.contiguous().requires_grad_()
+        ids, logits = t[:, None], torch.zeros(70, 1, device="cuda")
+        ops = torch.ops.aster_b200
+        forms = {"function": (lambda: hl.linear_distillation(x, w, logits, ids)) if distill else (lambda: hl.linear_cross_entropy(x, w, t)),
+                 "operator": (lambda: ops.linear_distillation(x, w, logits, ids)[0]) if distill else (lambda: ops.linear_cross_entropy(x, w, t)[0])}
+        forms[captured]()  # the first call on a device comes before a capture
+        alive = forms[eager]()
+        with pytest.raises(RuntimeError, match="still alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                forms[captured]()
+        want = torch.autograd.grad(alive, (x, w))
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(forms[captured](), (x, w))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
