@@ -72,7 +72,8 @@ __device__ __forceinline__ long long load_index(const void* p, int bits, size_t 
 
 // One block per row: the teacher's probabilities over its listed entries, sorted by id (a bitonic network over
 // the next power of two `n`; the key's low half is the listing order, so that equal ids stay in it and no two
-// keys are equal).
+// keys are equal).  The temperature divides differences to the row's maximum, never the logits themselves: those
+// may be as large as fp32 goes (masks of the type's lowest value), and minus infinity alone leaves an entry out.
 __global__ void __launch_bounds__(kMaxTop / 2) teacher_kernel(const void* __restrict__ logits, int dtype, const void* __restrict__ ids_in, int bits, int top, int n,
                                                               int vocab, float inv_t, int32_t* __restrict__ ids, float* __restrict__ probs,
                                                               float* __restrict__ weight, float* __restrict__ neg_entropy) {
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(kMaxTop / 2) teacher_kernel(const void* __rest
     uint32_t id32 = head::kNoLabel;
     if (j < top) {
       const long long id = load_index(ids_in, bits, base + j);
-      float t = load_float(logits, dtype, base + j) * inv_t;
+      float t = load_float(logits, dtype, base + j);
       const bool listed = id >= 0 && t != -INFINITY;
       if (listed) {
         any = 1;
@@ -106,7 +107,7 @@ __global__ void __launch_bounds__(kMaxTop / 2) teacher_kernel(const void* __rest
   bad = __syncthreads_or(bad);
   mx = block_reduce(mx, true, buf);
   float sum = 0.0f;
-  for (int j = threadIdx.x; j < top; j += blockDim.x) sum += any ? expf(s_t[j] - mx) : 0.0f;
+  for (int j = threadIdx.x; j < top; j += blockDim.x) sum += any ? expf((s_t[j] - mx) * inv_t) : 0.0f;
   sum = block_reduce(sum, false, buf);
   for (int size = 2; size <= n; size <<= 1) {
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(kMaxTop / 2) teacher_kernel(const void* __rest
   for (int place = threadIdx.x; place < top; place += blockDim.x) {
     const uint64_t k = key[place];
     const int32_t id = static_cast<int32_t>(k >> 32);
-    const float d = s_t[static_cast<uint32_t>(k)] - mx;
+    const float d = (s_t[static_cast<uint32_t>(k)] - mx) * inv_t;
     const float p = id != head::kNoLabel ? expf(d) * inv : 0.0f;
     ids[base + place] = id;
     probs[base + place] = p;

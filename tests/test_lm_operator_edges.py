@@ -8,6 +8,7 @@ import aster_b200.torch_op as top
 from aster_b200 import dtypes
 from aster_b200 import head_loss as hl
 from aster_b200.gemm import gemm
+from test_head_loss import distill_reference, make, teacher
 
 BF16 = torch.bfloat16
 
@@ -180,3 +181,25 @@ class TestCaptureBesideAGraph:
             got = torch.autograd.grad(forms[captured](), (x, w))
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+class TestEndsOfTheRange:
+    @pytest.mark.parametrize("teacher_dtype", [torch.float32, BF16, torch.float16])
+    @pytest.mark.parametrize("tau", [0.5, 1.0, 3.0])
+    def test_teacher_logits_as_large_as_their_type(self, gpu, teacher_dtype, tau):
+        """Only minus infinity leaves an entry out: the type's lowest value is an entry without weight, or with
+        the same weight as its neighbours where a row holds nothing else."""
+        x, w, g = make(40, 64, 300, BF16, 61)
+        ids, logits = teacher(40, 300, 6, g, teacher_dtype)
+        lowest, largest = torch.finfo(teacher_dtype).min, torch.finfo(teacher_dtype).max
+        ids[4:12] = torch.arange(6, device="cuda") * 7
+        logits[4:7, :4], logits[7:9], logits[9:11, 2], logits[11, :] = lowest, lowest, largest, largest
+        logits[4:7, 4:], logits[9:11, :2], logits[9:11, 3:] = 0.25, 1.0, lowest
+        ref = distill_reference(x, w, logits, ids, tau, reduction="none")
+        x.requires_grad_(), w.requires_grad_()
+        loss = hl.linear_distillation(x, w, logits, ids, temperature=tau, reduction="none")
+        ref.check_loss(loss)
+        ref.check_grads(*torch.autograd.grad(loss.sum(), (x, w)))
+        ref = distill_reference(x.detach(), w.detach(), logits, ids, tau)
+        ref.check_loss(hl.linear_distillation(x, w, logits, ids, temperature=tau))
