@@ -405,7 +405,8 @@ int make_plan(const b200_head_desc& d, Plan* p) {
   if (d.kind == B200_HEAD_DISTILL) {
     B200_REQUIRE(d.top >= 1 && d.top <= kMaxTop, "head_loss: top=%d outside [1, %d]", d.top, kMaxTop);
     B200_REQUIRE(d.dtype_teacher == B200_F32 || d.dtype_teacher == B200_BF16 || d.dtype_teacher == B200_F16, "head_loss: dtype_teacher=%d is not f32, bf16 or f16", d.dtype_teacher);
-    B200_REQUIRE(d.temperature > 0.0f && d.temperature < INFINITY, "head_loss: temperature must be positive and finite");
+    // 1 / T and T^2 have to be numbers that fp32 holds in full.
+    B200_REQUIRE(d.temperature >= 0x1p-60f && d.temperature <= 0x1p60f, "head_loss: temperature=%g is outside [2^-60, 2^60]", d.temperature);
   } else {
     B200_REQUIRE(d.label_smoothing >= 0.0f && d.label_smoothing < 1.0f, "head_loss: label_smoothing must be in [0, 1)");
   }

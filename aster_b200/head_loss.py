@@ -181,8 +181,8 @@ def _distill_head(x, w, teacher_logits, teacher_ids, temperature, reduction, gra
         if teacher_logits.dtype not in _TEACHER_DTYPES:
             raise RuntimeError(f"unsupported teacher_logits dtype {teacher_logits.dtype}")
         teacher_logits = teacher_logits.detach().contiguous()
-    if not 0.0 < temperature < float("inf"):
-        raise RuntimeError(f"temperature={temperature} must be positive and finite")
+    if not 2.0 ** -60 <= temperature <= 2.0 ** 60:  # 1 / T and T^2 are fp32 numbers in full
+        raise RuntimeError(f"temperature={temperature} is outside [2^-60, 2^60]")
     return _Head(x, w, teacher_ids, reduction, kind=nat.HEAD_DISTILL, temperature=temperature, teacher=teacher_logits, grad_bytes=grad_bytes)
 
 

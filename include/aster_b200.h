@@ -351,7 +351,7 @@ typedef struct b200_head_desc {
   int32_t top;                 /* distillation: entries per row, 1..1024                        */
   int32_t dtype_teacher;       /* distillation: B200_F32 | B200_BF16 | B200_F16                 */
   float label_smoothing;       /* cross entropy: [0, 1)                                         */
-  float temperature;           /* distillation: > 0                                             */
+  float temperature;           /* distillation: 2^-60 .. 2^60                                   */
   int64_t grad_bytes;          /* limit of the stored range of dL/dz; 0 = 256 MiB               */
 } b200_head_desc;
 

@@ -5,9 +5,11 @@ import pytest
 import torch
 
 import aster_b200.torch_op as top
+from aster_b200 import _native as nat
 from aster_b200 import dtypes
 from aster_b200 import head_loss as hl
 from aster_b200.gemm import gemm
+import test_head_loss as basics
 from test_head_loss import distill_reference, make, teacher
 
 BF16 = torch.bfloat16
@@ -181,6 +183,38 @@ class TestCaptureBesideAGraph:
             got = torch.autograd.grad(forms[captured](), (x, w))
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+class TestTemperatures:
+    """1 / T and T^2 leave fp32 long before T does."""
+
+    def test_extremes_are_refused(self, native_lib):
+        for tau in (1e-45, 1e-40, 1e-30, 2.0 ** -61, 2.0 ** 61, 1e25, 3e38):
+            with pytest.raises(nat.B200Error, match="temperature"):
+                hl._sizes(basics.TestOnHost.desc(kind=nat.HEAD_DISTILL, temperature=tau))
+        for tau in (2.0 ** -60, 1e-3, 2.0 ** 60):
+            hl._sizes(basics.TestOnHost.desc(kind=nat.HEAD_DISTILL, temperature=tau))
+
+    @pytest.mark.gpu
+    def test_extremes_are_refused_on_tensors(self, gpu):
+        x, w, t = strided_problem("cuda")
+        for tau in (1e-30, 1e-50, 1e25, 1e50):
+            with pytest.raises(RuntimeError, match="temperature"):
+                hl.linear_distillation(x, w, torch.zeros(70, 1, device="cuda"), t[:, None], temperature=tau)
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("tau", [2.0 ** -20, 2.0 ** 20])
+    def test_far_from_one(self, gpu, tau):
+        """Finite, and the limit's value: one certain entry's distance to the largest logit, or the entropies' difference."""
+        x, w, g = make(40, 64, 300, BF16, 62)
+        ids = torch.randint(0, 300, (40, 1), device="cuda", generator=g)
+        loss = hl.linear_distillation(x, w, torch.zeros(40, 1, device="cuda"), ids, temperature=tau, reduction="none")
+        z = x.double() @ w.double().T / tau
+        want = tau * tau * (torch.logsumexp(z, 1) - z.gather(1, ids)[:, 0])
+        # a logit is off by 5 roundings of at most 2^-23 of |x| . |w|, twice; lse and z each by half a step of 2^-24
+        dz = 5 * 2.0 ** -23 * (x.double().abs() @ w.double().abs().T).amax(1) / tau
+        bound = tau * tau * (2 * dz + 2.0 ** -16 + 2.0 ** -22 * z.abs().amax(1))
+        assert bool(((loss.double() - want).abs() <= bound).all())
 
 
 @pytest.mark.gpu
