@@ -43,6 +43,7 @@ constexpr int kThreads = 192;
 constexpr int kEpilogueWarps = 4;
 constexpr unsigned long long kWaitTimeoutNs = 2000000000ull;  // 2 s
 constexpr unsigned long long kDrainTimeoutNs = 20000000ull;   // 20 ms
+constexpr unsigned long long kSettleNs = 1000000ull;          // 1 ms, a thousand times what a copy takes
 
 // Status codes (status[0]); status[1] = blockIdx.x, status[2] = tile, status[3] = k block.
 // status[4..5] = SM cycles and status[6..7] = nanoseconds that CTA 0 spent in the kernel (the
@@ -252,6 +253,13 @@ struct Waiter {
     return ok != 0;
   }
 
+  // Aborting, the second CTA of a pair: its copies report to the leader's barriers, which may wait for fewer of
+  // them than were issued here.  Time for the last ones to land.
+  __device__ __noinline__ void settle() const {
+    unsigned long long t0 = sm100::globaltimer_ns();
+    while (!wait_expired(t0, kSettleNs)) __nanosleep(1000);
+  }
+
   __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, uint32_t code, int tile, int kb,
                                          unsigned long long limit) const {
     unsigned long long t0 = sm100::globaltimer_ns();
@@ -259,7 +267,7 @@ struct Waiter {
     for (uint32_t spin = 1;; ++spin) {
       if (sm100::mbar_try_wait(bar, parity)) return true;
       if ((spin & 63u) == 0u) {
-        if (*abort_flag != 0u) return false;
+        if (code != 0u && *abort_flag != 0u) return false;  // code 0: the waits of an abort itself, for copies and MMAs in flight
         if (wait_expired(t0, limit)) {
           if (code != 0u && atomicCAS(status, 0u, code) == 0u) {
             status[1] = blockIdx.x;
@@ -700,6 +708,8 @@ gemm_tn_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           waiter.wait(full_bar(s), static_cast<uint32_t>((last / p.stages) & 1), 0u, 0, 0, kDrainTimeoutNs);
         }
       }
+    } else if (!ok) {
+      waiter.settle();
     }
   } else if (warp == 1) {
     // ------------------------------- MMA issuer (leader CTA only) -------------------------------

@@ -537,6 +537,8 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
           waiter.wait(full_bar(s), static_cast<uint32_t>((last / p.stages) & 1), 0u, 0, 0, gemm::kDrainTimeoutNs);
         }
       }
+    } else if (!ok) {
+      waiter.settle();
     }
   } else if (warp == 1) {
     // ------------------------------- MMA issuer (leader CTA only) -------------------------------

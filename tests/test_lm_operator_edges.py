@@ -8,7 +8,7 @@ import aster_b200.torch_op as top
 from aster_b200 import _native as nat
 from aster_b200 import dtypes
 from aster_b200 import head_loss as hl
-from aster_b200.gemm import gemm
+from aster_b200.gemm import GemmPlan, gemm
 import test_head_loss as basics
 from test_head_loss import distill_reference, make, teacher
 
@@ -237,3 +237,27 @@ class TestEndsOfTheRange:
         ref.check_grads(*torch.autograd.grad(loss.sum(), (x, w)))
         ref = distill_reference(x.detach(), w.detach(), logits, ids, tau)
         ref.check_loss(hl.linear_distillation(x, w, logits, ids, temperature=tau))
+
+
+@pytest.mark.gpu
+class TestWaitsThatRunOut:
+    @pytest.mark.parametrize("dtype", ["bf16", "mxe2m1"])
+    @pytest.mark.parametrize("cta_group", [1, 2])
+    def test_an_abort_waits_for_its_own_copies(self, gpu, dtype, cta_group):
+        """No stage is handed over (the plan's own switch for this test): after the wait limit the producer waits
+        for each of its four slots, 20 ms at most, instead of leaving at once because the CTA is aborting."""
+        import time
+
+        plan = GemmPlan(512, 256, 8192, dtype, "f32", cta_group=cta_group, tile_n=128, stages=4, debug_mode=8, wait_limit_ms=20)
+        a, b, c = (torch.zeros(512 * 8192, dtype=torch.bfloat16, device="cuda") for _ in range(3))
+        scales = torch.full((1 << 20,), 127, dtype=torch.uint8, device="cuda")
+        if dtype == "mxe2m1":
+            plan.set_mx_scales(scales.data_ptr(), scales.data_ptr())
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        plan.run(a.data_ptr(), b.data_ptr(), c.data_ptr())
+        with pytest.raises(nat.B200Error, match="code 0x"):
+            plan.status()
+        elapsed = time.perf_counter() - t0
+        assert 0.02 + 4 * 0.02 <= elapsed < 1.0
+        assert plan.status() == [0, 0, 0, 0]
