@@ -128,6 +128,8 @@ class HeadDesc(C.Structure):
         ("label_smoothing", C.c_float),
         ("temperature", C.c_float),
         ("grad_bytes", C.c_int64),
+        ("wait_limit_ms", C.c_int32),
+        ("reserved", C.c_int32),
     ]
 
 

@@ -69,8 +69,8 @@ struct Problem {
   FastDiv group;     // raster_group
   FastDiv last_group;  // m-blocks of the last raster group
   int a_mn, b_mn;    // operand lies with its rows along K
-  int a_row0, b_row0;  // first row of A / B in their tensor maps
-  int a_k0, b_k0;    // first K coordinate in their tensor maps
+  int b_row0;        // first row of B in its tensor map
+  int b_k0;          // first K coordinate of B in its tensor map
   uint32_t idesc;
   // kProduct
   void* out16;       // [M][ld], or null: fp32 partial sums
@@ -87,7 +87,7 @@ struct Params {
   int stages;
   int extra_rounds;  // see Walk
   uint32_t* status;
-  unsigned wait_limit_ms;
+  unsigned wait_limit_ms;  // 0 = gemm::kWaitTimeoutNs
   // labels: `top` entries per row in rising order of their ids (top = 1: the target itself)
   int tokens, vocab;
   int col0;          // first column of the vocabulary in this launch (kGrad)
@@ -139,6 +139,10 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// Has a bounded wait given up since the status words were last read?  What it left out is then missing from the
+// sums of the kernels that follow: their results are made NaN.
+__device__ __forceinline__ bool wait_lost(const uint32_t* status) { return *reinterpret_cast<const volatile uint32_t*>(status) != gemm::kStatusOk; }
 
 // Four MMAs of one stage; `a_step` / `b_step` advance an operand's descriptor by 16 elements of K.
 #define B200_HEAD_STAGE_ASM(GROUP)                                                              \
@@ -483,7 +487,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
       const CUtensorMap* mb = MODE == kProduct && w.prob ? &map_b1 : &map_b0;
       const bool a_mn = MODE == kProduct && q.a_mn != 0;
       const bool b_mn = MODE == kProduct && q.b_mn != 0;
-      const int a_row = q.a_row0 + w.m_blk * kTileM + static_cast<int>(cta_rank) * kBM;
+      const int a_row = w.m_blk * kTileM + static_cast<int>(cta_rank) * kBM;
       const int b_row = q.b_row0 + w.n_blk * p.bn + static_cast<int>(cta_rank * b_rows);
       for (int kb = 0; kb < w.nkb; ++kb) {
         if (!waiter.wait(empty_bar(stage), phase ^ 1u, gemm::kStatusProducerEmptyWait, item, kb)) {
@@ -493,7 +497,7 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
         if (elect_one()) {
           const uint32_t a_dst = smem_base + static_cast<uint32_t>(stage) * st_bytes;
           const uint32_t b_dst = a_dst + a_bytes;
-          const int ka = q.a_k0 + (w.kb0 + kb) * kStageK;
+          const int ka = (w.kb0 + kb) * kStageK;
           const int kbq = q.b_k0 + (w.kb0 + kb) * kStageK;
           uint32_t bar = full_bar(stage);
           if constexpr (CG == 1) {
@@ -611,7 +615,10 @@ head_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ 
     [[maybe_unused]] const TurnAround turn{turn_base + static_cast<uint32_t>(warp - 2) * kTurnBytes};
     const int row_in_tile = static_cast<int>(cta_rank) * kBM + quarter * 32 + lane;
     float unscale = 1.0f;
-    if constexpr (MODE == kProduct) unscale = p.unscale != nullptr ? __ldg(p.unscale) : __ldg(p.share) * __ldg(p.grad_loss) * p.unscale_factor;
+    if constexpr (MODE == kProduct) {
+      unscale = p.unscale != nullptr ? __ldg(p.unscale) : __ldg(p.share) * __ldg(p.grad_loss) * p.unscale_factor;
+      if (wait_lost(p.status)) unscale = NAN;  // z or G are not what they should be
+    }
     int acc = 0;
     uint32_t acc_phase = 0;
     for (Walk walk(p, unit, units);;) {

@@ -158,6 +158,7 @@ struct JoinParams {
   float* share;              // what a row's gradient is divided by, as a factor
   float2* block_sums;
   uint32_t* ticket;
+  const uint32_t* status;
 };
 
 // 8 rows per block of 8 warps.  A thread joins every 32nd tile of one row (8 lanes read 8 neighbouring rows
@@ -171,6 +172,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) 
   __shared__ uint32_t s_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   sm100::griddep_wait();
+  const bool lost = head::wait_lost(p.status);
   {
     const int r = threadIdx.x % kJoinRows, group = threadIdx.x / kJoinRows;
     const int row = blockIdx.x * kJoinRows + r;
@@ -226,6 +228,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) 
         kept = 1.0f;
       }
     }
+    if (lost) loss = NAN;
     if (lane == 0) {
       p.lse[row] = lse;
       if (p.reduction == B200_REDUCE_NONE) p.loss[row] = loss;
@@ -279,7 +282,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) 
     }
     const bool mean = p.reduction == B200_REDUCE_MEAN;
     *p.loss = static_cast<float>(mean ? a / k : a);
-    *p.share = !mean ? 1.0f : (k > 0.0 ? static_cast<float>(1.0 / k) : 0.0f);  // without any row the gradients are zero
+    *p.share = lost ? NAN : !mean ? 1.0f : (k > 0.0 ? static_cast<float>(1.0 / k) : 0.0f);  // without any row the gradients are zero
   }
 }
 
@@ -319,14 +322,16 @@ __global__ void __launch_bounds__(1024) factor_kernel(const float* __restrict__ 
 
 // A gradient as the sum of its fp32 parts, in their order, rounded once.  n4 = elements / 4.
 template <typename T16>
-__global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ parts, int splits, size_t n4, T16* __restrict__ out) {
+__global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ parts, int splits, size_t n4, T16* __restrict__ out, const uint32_t* status) {
   sm100::griddep_wait();
+  const float lost = head::wait_lost(status) ? NAN : 0.0f;
   for (size_t i = static_cast<size_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n4; i += static_cast<size_t>(gridDim.x) * blockDim.x) {
     float4 a = __ldcs(reinterpret_cast<const float4*>(parts) + i);
     for (int s = 1; s < splits; ++s) {
       const float4 b = __ldcs(reinterpret_cast<const float4*>(parts) + s * n4 + i);
       a = make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
     }
+    if (lost != 0.0f) a = make_float4(lost, lost, lost, lost);
     reinterpret_cast<uint2*>(out)[i] = make_uint2(head::pack2<T16>(a.x, a.y), head::pack2<T16>(a.z, a.w));
   }
 }
@@ -402,6 +407,7 @@ int make_plan(const b200_head_desc& d, Plan* p) {
   B200_REQUIRE(d.reduction >= B200_REDUCE_NONE && d.reduction <= B200_REDUCE_SUM, "head_loss: reduction=%d", d.reduction);
   B200_REQUIRE(d.index_bits == 32 || d.index_bits == 64, "head_loss: index_bits=%d is not 32 or 64", d.index_bits);
   B200_REQUIRE(d.grad_bytes >= 0, "head_loss: grad_bytes must be >= 0");
+  B200_REQUIRE(d.wait_limit_ms >= 0, "head_loss: wait_limit_ms must be >= 0");
   if (d.kind == B200_HEAD_DISTILL) {
     B200_REQUIRE(d.top >= 1 && d.top <= kMaxTop, "head_loss: top=%d outside [1, %d]", d.top, kMaxTop);
     B200_REQUIRE(d.dtype_teacher == B200_F32 || d.dtype_teacher == B200_BF16 || d.dtype_teacher == B200_F16, "head_loss: dtype_teacher=%d is not f32, bf16 or f16", d.dtype_teacher);
@@ -592,11 +598,11 @@ int launch_small(void (*fn)(Args...), unsigned grid, unsigned threads, size_t sm
   return B200_OK;
 }
 
-int launch_sum_parts(int dtype, const float* parts, int splits, size_t n, void* out, cudaStream_t stream) {
+int launch_sum_parts(int dtype, const float* parts, int splits, size_t n, void* out, const uint32_t* status, cudaStream_t stream) {
   const size_t n4 = n / 4;
   const unsigned blocks = static_cast<unsigned>(std::min<size_t>((n4 + 255) / 256, kSms * 8));
-  if (dtype == B200_F16) return launch_small(sum_parts_kernel<__half>, blocks, 256u, 0u, stream, parts, splits, n4, static_cast<__half*>(out));
-  return launch_small(sum_parts_kernel<__nv_bfloat16>, blocks, 256u, 0u, stream, parts, splits, n4, static_cast<__nv_bfloat16*>(out));
+  if (dtype == B200_F16) return launch_small(sum_parts_kernel<__half>, blocks, 256u, 0u, stream, parts, splits, n4, static_cast<__half*>(out), status);
+  return launch_small(sum_parts_kernel<__nv_bfloat16>, blocks, 256u, 0u, stream, parts, splits, n4, static_cast<__nv_bfloat16*>(out), status);
 }
 
 // z = x . w^T over the columns [col0, col0 + cols).
@@ -628,6 +634,7 @@ int set_items(Problem* q) {
 void set_labels(const b200_head_desc& d, const Plan& pl, const void* labels, const void* saved, uint32_t* status, Params* p) {
   std::memset(p, 0, sizeof(*p));
   p->status = status;
+  p->wait_limit_ms = static_cast<unsigned>(d.wait_limit_ms);
   p->num_probs = 1;
   p->tokens = static_cast<int>(d.tokens);
   p->vocab = static_cast<int>(d.vocab);
@@ -754,6 +761,7 @@ int b200_head_loss_forward(const b200_head_desc* desc, const void* x, const void
   j.share = reinterpret_cast<float*>(sv);
   j.block_sums = reinterpret_cast<float2*>(ws + pl.f_sums);
   j.ticket = p.ticket;
+  j.status = status;
   return launch_small(join_kernel, static_cast<unsigned>(div_up(d.tokens, kJoinRows)), kJoinThreads, 0u, s, j);
 }
 
@@ -822,6 +830,7 @@ int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const voi
     Params q;
     std::memset(&q, 0, sizeof(q));
     q.status = status;
+    q.wait_limit_ms = static_cast<unsigned>(d.wait_limit_ms);
     q.unscale = per_row ? unscale : nullptr;
     q.share = share;
     q.grad_loss = grad_loss;
@@ -878,12 +887,12 @@ int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const voi
     if (rc != B200_OK) return rc;
     if (grad_w != nullptr && pl.w_splits > 1) {
       rc = launch_sum_parts(d.dtype, reinterpret_cast<const float*>(ws + pl.b_w_parts), pl.w_splits, static_cast<size_t>(cols) * static_cast<size_t>(d.hidden),
-                            static_cast<uint8_t*>(grad_w) + static_cast<size_t>(col0) * d.hidden * 2, s);
+                            static_cast<uint8_t*>(grad_w) + static_cast<size_t>(col0) * d.hidden * 2, status, s);
       if (rc != B200_OK) return rc;
     }
   }
   if (grad_x != nullptr && !pl.direct) {
-    return launch_sum_parts(d.dtype, parts, pl.splits, static_cast<size_t>(d.tokens) * static_cast<size_t>(d.hidden), grad_x, s);
+    return launch_sum_parts(d.dtype, parts, pl.splits, static_cast<size_t>(d.tokens) * static_cast<size_t>(d.hidden), grad_x, status, s);
   }
   return B200_OK;
 }

@@ -273,7 +273,8 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: t
 
 def head_loss_status() -> Sequence[int]:
     """Status words of the calls made so far on the current device (synchronises it); raises
-    ``B200Error`` (TIMEOUT) if a bounded device-side wait gave up."""
+    ``B200Error`` (TIMEOUT) if a bounded device-side wait gave up.  From then until this call, losses
+    and gradients on that device are NaN."""
     words = (C.c_uint32 * 4)()
     nat.call("b200_head_loss_status", words)
     return list(words)

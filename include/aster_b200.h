@@ -353,6 +353,8 @@ typedef struct b200_head_desc {
   float label_smoothing;       /* cross entropy: [0, 1)                                         */
   float temperature;           /* distillation: 2^-60 .. 2^60                                   */
   int64_t grad_bytes;          /* limit of the stored range of dL/dz; 0 = 256 MiB               */
+  int32_t wait_limit_ms;       /* limit of the device-side waits; 0 = 2000                      */
+  int32_t reserved;
 } b200_head_desc;
 
 typedef struct b200_head_sizes {
@@ -371,7 +373,9 @@ int b200_head_loss_forward(const b200_head_desc* desc, const void* x, const void
 int b200_head_loss_backward(const b200_head_desc* desc, const void* x, const void* w, const void* labels, const float* lse, const void* saved,
                             const float* grad_loss, void* grad_x, void* grad_w, void* workspace, size_t workspace_bytes, void* stream);
 /* Did every bounded device-side wait of the calls made so far on the current device complete?
- * (Synchronises it.)  words[0] = 0, else a code naming the wait and B200_ERR_TIMEOUT. */
+ * (Synchronises it.)  words[0] = 0, else a code naming the wait and B200_ERR_TIMEOUT.  From such a wait until
+ * this call, losses and gradients on the device come out as NaN (but for gradients that the launch which gave
+ * up wrote itself). */
 int b200_head_loss_status(uint32_t words[4]);
 
 /* ---- optional: gather row shards of C onto every GPU (NCCL over NVLink) ------------------

@@ -261,3 +261,32 @@ class TestWaitsThatRunOut:
         elapsed = time.perf_counter() - t0
         assert 0.02 + 4 * 0.02 <= elapsed < 1.0
         assert plan.status() == [0, 0, 0, 0]
+
+    @pytest.mark.parametrize("T", [100, 256])  # one CTA, a pair
+    def test_a_loss_whose_product_gave_up_is_nan(self, gpu, T):
+        """A product of two tiles with 65536 K blocks each (several milliseconds) under a limit of 1 ms: the status
+        names the wait, losses and gradients are NaN until it is read, and the next call is right again."""
+        x, w, g = make(T, 64, 128, BF16, 71)
+        t = torch.randint(0, 128, (T,), device="cuda", generator=g)
+        x.requires_grad_(), w.requires_grad_()
+        before = hl.linear_cross_entropy(x, w, t)
+        want = torch.autograd.grad(before, (x, w))
+        before = hl.linear_cross_entropy(x, w, t)  # a graph from before the lost wait
+        rows = hl.linear_cross_entropy(x, w, t, reduction="none")
+        long_x, long_w = (torch.zeros(n, 1 << 22, dtype=BF16, device="cuda") for n in (T, 128))
+        for reduction in ("mean", "none"):
+            assert hl.head_loss_status() == [0, 0, 0, 0]
+            slow = hl._xent_head(long_x, long_w, t, -100, 0.0, reduction)
+            slow.desc.wait_limit_ms = 1
+            loss, _, _ = slow.forward()
+            assert bool(torch.isnan(loss).all())
+            assert bool(torch.isnan(hl.linear_cross_entropy(x, w, t)))
+            for kept in (before, rows.sum()):
+                assert all(bool(torch.isnan(v).all()) for v in torch.autograd.grad(kept, (x, w), retain_graph=True))
+            with pytest.raises(nat.B200Error, match="code 0x"):
+                hl.head_loss_status()
+        del long_x, long_w, slow
+        after = hl.linear_cross_entropy(x, w, t)
+        got = torch.autograd.grad(after, (x, w))
+        assert torch.equal(after, before) and all(torch.equal(a, b) for a, b in zip(got, want))
+        assert hl.head_loss_status() == [0, 0, 0, 0]
