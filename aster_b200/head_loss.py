@@ -290,6 +290,15 @@ def _align256(n: int) -> int:
     return (n + 255) // 256 * 256
 
 
+def _wanted(x, weight, dx, dw, want_x: bool, want_w: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """Both gradients of an operator, which cannot return None: an unwanted one is empty."""
+    return dx.view(x.shape) if want_x else x.new_empty(0), dw if want_w else weight.new_empty(0)
+
+
+def _fake_wanted(x, weight, want_x: bool, want_w: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    return x.new_empty(x.shape if want_x else 0), weight.new_empty(weight.shape if want_w else 0)
+
+
 @torch.library.custom_op("aster_b200::linear_cross_entropy", mutates_args=())
 def _xent_op(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100, label_smoothing: float = 0.0,
              reduction: str = "mean") -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -305,14 +314,14 @@ def _(x, weight, target, ignore_index=-100, label_smoothing=0.0, reduction="mean
 
 @torch.library.custom_op("aster_b200::linear_cross_entropy_backward", mutates_args=())
 def _xent_backward_op(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, saved: torch.Tensor,
-                      ignore_index: int, label_smoothing: float, reduction: str) -> tuple[torch.Tensor, torch.Tensor]:
-    dx, dw = _xent_head(x, weight, target, ignore_index, label_smoothing, reduction).backward(grad, lse, saved, True, True)
-    return dx.view(x.shape), dw
+                      ignore_index: int, label_smoothing: float, reduction: str, want_x: bool = True, want_w: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    dx, dw = _xent_head(x, weight, target, ignore_index, label_smoothing, reduction).backward(grad, lse, saved, want_x, want_w)
+    return _wanted(x, weight, dx, dw, want_x, want_w)
 
 
 @_xent_backward_op.register_fake
-def _(grad, x, weight, target, lse, saved, ignore_index, label_smoothing, reduction):
-    return x.new_empty(x.shape), weight.new_empty(weight.shape)
+def _(grad, x, weight, target, lse, saved, ignore_index, label_smoothing, reduction, want_x=True, want_w=True):
+    return _fake_wanted(x, weight, want_x, want_w)
 
 
 def _watch_operator(ctx, x: torch.Tensor, w: torch.Tensor) -> None:
@@ -328,8 +337,9 @@ def _xent_setup(ctx, inputs, output):
 
 
 def _xent_autograd(ctx, grad, _lse, _saved):
-    dx, dw = torch.ops.aster_b200.linear_cross_entropy_backward(grad, *ctx.saved_tensors, ctx.ignore_index, ctx.label_smoothing, ctx.reduction)
-    return dx, dw, None, None, None, None
+    want_x, want_w = ctx.needs_input_grad[:2]
+    dx, dw = torch.ops.aster_b200.linear_cross_entropy_backward(grad, *ctx.saved_tensors, ctx.ignore_index, ctx.label_smoothing, ctx.reduction, want_x, want_w)
+    return dx if want_x else None, dw if want_w else None, None, None, None, None
 
 
 _xent_op.register_autograd(_xent_autograd, setup_context=_xent_setup)
@@ -351,14 +361,14 @@ def _(x, weight, teacher_logits, teacher_ids, temperature=1.0, reduction="mean")
 
 @torch.library.custom_op("aster_b200::linear_distillation_backward", mutates_args=())
 def _distill_backward_op(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, lse: torch.Tensor, saved: torch.Tensor,
-                         temperature: float, reduction: str) -> tuple[torch.Tensor, torch.Tensor]:
-    dx, dw = _distill_head(x, weight, None, teacher_ids, temperature, reduction).backward(grad, lse, saved, True, True)
-    return dx.view(x.shape), dw
+                         temperature: float, reduction: str, want_x: bool = True, want_w: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    dx, dw = _distill_head(x, weight, None, teacher_ids, temperature, reduction).backward(grad, lse, saved, want_x, want_w)
+    return _wanted(x, weight, dx, dw, want_x, want_w)
 
 
 @_distill_backward_op.register_fake
-def _(grad, x, weight, teacher_ids, lse, saved, temperature, reduction):
-    return x.new_empty(x.shape), weight.new_empty(weight.shape)
+def _(grad, x, weight, teacher_ids, lse, saved, temperature, reduction, want_x=True, want_w=True):
+    return _fake_wanted(x, weight, want_x, want_w)
 
 
 def _distill_setup(ctx, inputs, output):
@@ -369,8 +379,9 @@ def _distill_setup(ctx, inputs, output):
 
 
 def _distill_autograd(ctx, grad, _lse, _saved):
-    dx, dw = torch.ops.aster_b200.linear_distillation_backward(grad, *ctx.saved_tensors, ctx.temperature, ctx.reduction)
-    return dx, dw, None, None, None, None
+    want_x, want_w = ctx.needs_input_grad[:2]
+    dx, dw = torch.ops.aster_b200.linear_distillation_backward(grad, *ctx.saved_tensors, ctx.temperature, ctx.reduction, want_x, want_w)
+    return dx if want_x else None, dw if want_w else None, None, None, None, None
 
 
 _distill_op.register_autograd(_distill_autograd, setup_context=_distill_setup)

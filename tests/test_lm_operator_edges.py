@@ -290,3 +290,47 @@ class TestWaitsThatRunOut:
         got = torch.autograd.grad(after, (x, w))
         assert torch.equal(after, before) and all(torch.equal(a, b) for a, b in zip(got, want))
         assert hl.head_loss_status() == [0, 0, 0, 0]
+
+
+class TestOperatorsMakeWhatIsWanted:
+    """A frozen head or a frozen body costs the dispatcher's backward pass no gradient that nobody asked for."""
+
+    @staticmethod
+    def operators(x, w, t, logits):
+        ops = torch.ops.aster_b200
+        return lambda: ops.linear_cross_entropy(x, w, t)[0], lambda: ops.linear_distillation(x, w, logits, t[:, None])[0]
+
+    @pytest.mark.parametrize("which", [0, 1])
+    @pytest.mark.parametrize("want", ["x", "w", "both"])
+    def test_on_the_host(self, which, want):
+        from torch.utils._python_dispatch import TorchDispatchMode
+
+        class Record(TorchDispatchMode):
+            made = []
+
+            def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+                out = func(*args, **(kwargs or {}))
+                if "_backward" in str(func):
+                    self.made += [tuple(o.shape) for o in out]
+                return out
+
+        x, w, t = (v.to("meta") for v in strided_problem("cpu"))
+        x.requires_grad_(want != "w"), w.requires_grad_(want != "x")
+        loss = self.operators(x, w, t, torch.zeros(70, 1, device="meta"))[which]()
+        with Record() as record:
+            loss.backward()
+        assert record.made == [(0,) if want == "w" else (70, 136), (0,) if want == "x" else (300, 136)]
+        assert (x.grad is None) == (want == "w") and (w.grad is None) == (want == "x")
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("which", [0, 1])
+    def test_on_the_gpu(self, gpu, which):
+        x, w, t = strided_problem("cuda")
+        call = self.operators(x, w, t, torch.zeros(70, 1, device="cuda"))[which]
+        x.requires_grad_(), w.requires_grad_()
+        want = torch.autograd.grad(call(), (x, w))
+        for i, (leaf, other) in enumerate(((x, w), (w, x))):
+            other.requires_grad_(False)
+            got, = torch.autograd.grad(call(), leaf)
+            other.requires_grad_()
+            assert torch.equal(got, want[i])
