@@ -756,7 +756,9 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
   // between the CTAs of a cluster where that saves more than the 2.5 us of their exchange, as long as all of
   // them run at once (us, uncut or in two -> as chosen here: 1 x 1024 x 8192 10.6 -> 8.2,
   // 16 x 8192 x 16384 19.5 -> 17.6, 4 x 4096 x 16384 14.0 -> 13.5; 16 x 8192 x 8192 takes 12.0 with 128 uncut
-  // tiles of 64 columns, 12.5 with 64 of 128 cut in two).
+  // tiles of 64 columns, 12.5 with 64 of 128 cut in two).  A single K block leaves nothing to cut, and with many full
+  // tiles of it the outputs decide: 256 columns then take fewer starts (128 x 65536 x 256 in 128 / 256 columns 9.25 / 7.93,
+  // 65 x 131072 x 128 16.9 / 13.9, but 128 x 40000 x 256 7.4 / 7.7 and 64 x 65536 x 256 7.5 / 7.8).
   int mx4_bn = 0, mx4_cg = 0;
   if (mx == gemm::kMx4 && d.tile_n == 0 && d.M <= gemm::kBM && cg != 2) {
     cg = 1;
@@ -765,7 +767,7 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
     for (int parts : {1, 2, 4}) {
       for (int bn : {128, 64}) {
         const int64_t tiles = ceil_div(d.N, bn);
-        if (bn / parts < 32 || k_blocks < 2 * parts || (parts > 1 && tiles * parts > kDefaultSms)) continue;
+        if (parts > 1 && (bn / parts < 32 || k_blocks < 2 * parts || tiles * parts > kDefaultSms)) continue;
         const double compute_us = static_cast<double>((tiles * parts + kDefaultSms - 1) / kDefaultSms) * ceil_div(k_blocks, parts) * (bn == 64 ? 0.235 : 0.28);
         const double us = std::max(compute_us, dram_us) + (parts > 1 ? 2.5 : 0.0);
         if (mx4_bn == 0 || us < best - 1e-9) {
@@ -775,6 +777,7 @@ int b200_gemm_plan_create(const b200_gemm_desc* desc, b200_gemm_plan** out) {
         }
       }
     }
+    if (k_blocks == 1 && d.M > 64 && ceil_div(d.N, 128) > 3 * kDefaultSms) mx4_bn = 256;
   } else if (mx == gemm::kMx4 && d.tile_n == 0) {
     static const struct {
       int cg, bn;

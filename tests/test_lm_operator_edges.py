@@ -127,6 +127,31 @@ def exact_operand(rows, K, rng):
     return q, scales, dtypes.dequantize_mx(q, scales, "e2m1").astype(np.float64)
 
 
+class TestFewRowsShortK:
+    """One K block (K <= 256) is planned like several: narrow tiles for up to 128 rows."""
+
+    @pytest.mark.parametrize("K", [32, 96, 256])
+    @pytest.mark.parametrize("M", [1, 16, 60, 128])
+    @pytest.mark.parametrize("N", [64, 2048, 65536])
+    def test_plan(self, native_lib, M, N, K):
+        r = GemmPlan(M, N, K, "mxe2m1", "bf16").resources()
+        assert r.cta_group == 1 and r.tail_parts <= 1
+        if M > 64 and N > 3 * 148 * 128:  # full tiles in many rounds, whose outputs decide
+            assert r.tile_n == 256
+        else:
+            assert r.tile_n == GemmPlan(M, N, 288, "mxe2m1", "bf16").resources().tile_n and r.tile_n in (64, 128)
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("K", [32, 160, 256])
+    @pytest.mark.parametrize("M", [1, 40, 100, 128])
+    @pytest.mark.parametrize("N", [64, 263, 2048, 40000, 60000])
+    def test_exact_sums(self, gpu, M, N, K):
+        rng = np.random.default_rng(M + N + K)
+        (qa, sa, a), (qb, sb, b) = exact_operand(M, K, rng), exact_operand(N, K, rng)
+        got = gemm(qa, qb, dtype_ab="mxe2m1", dtype_c="f32", block_scales_a=sa, block_scales_b=sb)
+        assert np.array_equal(got, (a @ b.T).astype(np.float32))
+
+
 @pytest.mark.gpu
 class TestNanUnderRelu:
     @pytest.mark.parametrize("dtype_c", ["f32", "bf16"])
