@@ -32,6 +32,7 @@ import threading
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from .gemm import GemmPlan
@@ -237,11 +238,28 @@ def dequantize_mx_direct(q: torch.Tensor, scales: torch.Tensor, out_dtype: torch
     return out
 
 
+class _NoGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, out, bias):
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("aster_b200::gemm_mx_nt has no backward pass: its bias gets no gradient")
+
+
+def _without_gradient(out: torch.Tensor, bias: torch.Tensor) -> torch.Tensor:
+    """``out`` as part of ``bias``'s graph: a backward pass that reaches it is refused, as the dispatcher's form
+    does, where a result without a graph would leave the bias out of it silently."""
+    return _NoGradient.apply(out, bias)
+
+
 def gemm_mx_nt_direct(a: torch.Tensor, scales_a: torch.Tensor, b: torch.Tensor, scales_b: torch.Tensor, bias: Optional[torch.Tensor] = None,
                       relu: bool = False, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """``epilogue(A . B^T)`` of two block-scaled fp4 operands as :func:`quantize_mx_direct` returns
     them: ``a`` ``[M, K/2]``, ``b`` ``[N, K/2]``, optional float32 ``bias`` ``[N]`` and ReLU, fp32
-    accumulation, ``[M, N]`` out.  The first call of a shape allocates: inside a stream capture it is refused."""
+    accumulation, ``[M, N]`` out.  There is no backward pass: one that reaches the bias is refused.  The first
+    call of a shape allocates (its plan lives until :func:`clear_plan_cache`): inside a stream capture it is refused."""
     _check_mx_operand("a", a, scales_a)
     _check_mx_operand("b", b, scales_b)
     if a.device != b.device or a.shape[1] != b.shape[1]:
@@ -251,11 +269,13 @@ def gemm_mx_nt_direct(a: torch.Tensor, scales_a: torch.Tensor, b: torch.Tensor, 
     M, N, K = a.shape[0], b.shape[0], 2 * a.shape[1]
     if bias is not None and (bias.dtype != torch.float32 or bias.device != a.device or bias.numel() != N):
         raise RuntimeError(f"bias must be {N} float32 values on {a.device}")
+    if bias is not None and forward_ad.unpack_dual(bias).tangent is not None:
+        raise RuntimeError("aster_b200::gemm_mx_nt has no forward-mode derivative: bias must not carry a tangent")
     a, scales_a, b, scales_b = _aligned(a), _aligned(scales_a), _aligned(b), _aligned(scales_b)
     bias = None if bias is None else bias.contiguous()
     out = a.new_empty((M, N), dtype=out_dtype)
     _call(a.device, _gemm_mx, a, scales_a, b, scales_b, bias, relu, out)
-    return out
+    return _without_gradient(out, bias) if bias is not None and bias.requires_grad and torch.is_grad_enabled() else out
 
 
 def _gemm_mx(a, scales_a, b, scales_b, bias, relu, out, stream) -> int:

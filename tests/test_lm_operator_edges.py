@@ -359,3 +359,36 @@ class TestOperatorsMakeWhatIsWanted:
             got, = torch.autograd.grad(call(), leaf)
             other.requires_grad_()
             assert torch.equal(got, want[i])
+
+
+class TestProductHasNoBackward:
+    """A bias that wants a gradient is not left without one silently."""
+
+    def test_a_result_that_refuses_on_the_host(self):
+        out, bias = torch.zeros(3, 8), torch.zeros(8, requires_grad=True)
+        c = top._without_gradient(out, bias)
+        assert c.requires_grad and torch.equal(c.detach(), out)
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            c.sum().backward()
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("form", ["direct", "operator"])
+    def test_on_the_gpu(self, gpu, form):
+        q = top.quantize_mx_direct(torch.randn(40, 64, device="cuda"))
+        w = top.quantize_mx_direct(torch.randn(72, 64, device="cuda"))
+        bias = torch.randn(72, device="cuda")
+        call = top.gemm_mx_nt_direct if form == "direct" else torch.ops.aster_b200.gemm_mx_nt
+        want = call(*q, *w, bias)
+        assert not want.requires_grad
+        bias.requires_grad_()
+        got = call(*q, *w, bias)
+        with pytest.raises(RuntimeError, match="backward"):
+            got.sum().backward()
+        with torch.no_grad():
+            assert torch.equal(call(*q, *w, bias), want) and torch.equal(got, want)
+
+        from torch.autograd import forward_ad
+
+        bias.requires_grad_(False)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            call(*q, *w, forward_ad.make_dual(bias, bias))
