@@ -159,6 +159,10 @@ struct JoinParams {
   float2* block_sums;
   uint32_t* ticket;
   const uint32_t* status;
+  struct {
+    uint32_t* at;
+    int words;
+  } pad[4];                  // what lies between the parts of `saved`: it is an output, all of which is defined
 };
 
 // 8 rows per block of 8 warps.  A thread joins every 32nd tile of one row (8 lanes read 8 neighbouring rows
@@ -173,6 +177,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   sm100::griddep_wait();
   const bool lost = head::wait_lost(p.status);
+  if (blockIdx.x == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (static_cast<int>(threadIdx.x) < p.pad[i].words) p.pad[i].at[threadIdx.x] = 0u;  // fewer than 256 bytes
+    }
+  }
   {
     const int r = threadIdx.x % kJoinRows, group = threadIdx.x / kJoinRows;
     const int row = blockIdx.x * kJoinRows + r;
@@ -762,6 +772,17 @@ int b200_head_loss_forward(const b200_head_desc* desc, const void* x, const void
   j.block_sums = reinterpret_cast<float2*>(ws + pl.f_sums);
   j.ticket = p.ticket;
   j.status = status;
+  auto pad = [&](int i, size_t part, size_t words) {
+    const size_t end = part + words * 4;
+    j.pad[i] = {reinterpret_cast<uint32_t*>(sv + end), static_cast<int>((align256(end) - end) / 4)};
+  };
+  pad(0, 0, 1);
+  if (d.kind == B200_HEAD_DISTILL) {
+    const size_t rows = static_cast<size_t>(d.tokens), entries = rows * static_cast<size_t>(d.top);
+    pad(1, pl.s_weight, rows);
+    pad(2, pl.s_probs, entries);
+    pad(3, pl.s_ids, entries);
+  }
   return launch_small(join_kernel, static_cast<unsigned>(div_up(d.tokens, kJoinRows)), kJoinThreads, 0u, s, j);
 }
 

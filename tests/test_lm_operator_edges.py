@@ -392,3 +392,30 @@ class TestProductHasNoBackward:
         bias.requires_grad_(False)
         with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
             call(*q, *w, forward_ad.make_dual(bias, bias))
+
+
+@pytest.mark.gpu
+class TestOperatorsAsTorchKnowsThem:
+    def test_every_byte_of_the_outputs_is_defined(self, gpu):
+        """`saved` is an output, too: two calls give the same bytes, whatever was in the memory before."""
+        x, w, t = strided_problem("cuda")
+        ids, logits = torch.stack([t, (t + 7) % 300, torch.full_like(t, -1)], 1), torch.zeros(70, 3, device="cuda")
+        for call in (lambda: torch.ops.aster_b200.linear_cross_entropy(x, w, t), lambda: torch.ops.aster_b200.linear_distillation(x, w, logits, ids)):
+            outs = []
+            for fill in (0, 255, 7):
+                torch.cuda.synchronize()
+                torch.cuda.empty_cache()
+                torch.full((64 << 20,), fill, dtype=torch.uint8, device="cuda")  # what the allocator hands out next
+                outs.append(call())
+            assert all(torch.equal(a, b) for out in outs[1:] for a, b in zip(outs[0], out))
+
+    def test_opcheck(self, gpu):
+        from torch.library import opcheck
+
+        x, w, t = strided_problem("cuda")
+        ids, logits = t[:, None].contiguous(), torch.zeros(70, 1, device="cuda")
+        ops = torch.ops.aster_b200
+        for frozen in (None, x, w):
+            x.requires_grad_(frozen is not x), w.requires_grad_(frozen is not w)
+            opcheck(ops.linear_cross_entropy.default, (x, w, t, -100, 0.1, "none" if frozen is None else "mean"))
+            opcheck(ops.linear_distillation.default, (x, w, logits, ids, 2.0))
