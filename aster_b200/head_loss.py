@@ -255,6 +255,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     no gradient; any other target outside the vocabulary makes its loss, and the gradients it enters, NaN.
     "mean" divides by the number of targets that count (NaN without any).  ``grad_bytes`` limits what the
     backward pass keeps of ``dL/dz`` at a time (0: 256 MiB)."""
+    if torch.compiler.is_compiling():  # a compiler sees the operator, not what is behind it
+        return torch.ops.aster_b200.linear_cross_entropy(x, weight, target, ignore_index, label_smoothing, reduction, grad_bytes)[0]
     return _apply(x, weight, _xent_head(x, weight, target, ignore_index, label_smoothing, reduction, grad_bytes), target.shape)
 
 
@@ -268,6 +270,8 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_logits: t
     order, ``top`` at most 1024.  Entries with a negative id or a logit of minus infinity are left out; rows with
     nothing left have no loss and no gradient and do not count for "mean".  An id listed twice counts twice; an
     id beyond the vocabulary, or a logit that is NaN or plus infinity, makes the row NaN."""
+    if torch.compiler.is_compiling():
+        return torch.ops.aster_b200.linear_distillation(x, weight, teacher_logits, teacher_ids, temperature, reduction, grad_bytes)[0]
     return _apply(x, weight, _distill_head(x, weight, teacher_logits, teacher_ids, temperature, reduction, grad_bytes), teacher_ids.shape[:-1])
 
 
@@ -301,26 +305,27 @@ def _fake_wanted(x, weight, want_x: bool, want_w: bool) -> tuple[torch.Tensor, t
 
 @torch.library.custom_op("aster_b200::linear_cross_entropy", mutates_args=())
 def _xent_op(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100, label_smoothing: float = 0.0,
-             reduction: str = "mean") -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    head = _xent_head(x, weight, target, ignore_index, label_smoothing, reduction)
+             reduction: str = "mean", grad_bytes: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    head = _xent_head(x, weight, target, ignore_index, label_smoothing, reduction, grad_bytes)
     loss, lse, saved = head.forward()
     return loss.view(target.shape) if head.per_row else loss, lse, saved
 
 
 @_xent_op.register_fake
-def _(x, weight, target, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
+def _(x, weight, target, ignore_index=-100, label_smoothing=0.0, reduction="mean", grad_bytes=0):
     return _fake_outputs(x, reduction, target.shape, 256 if x.numel() else 0)
 
 
 @torch.library.custom_op("aster_b200::linear_cross_entropy_backward", mutates_args=())
 def _xent_backward_op(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, saved: torch.Tensor,
-                      ignore_index: int, label_smoothing: float, reduction: str, want_x: bool = True, want_w: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
-    dx, dw = _xent_head(x, weight, target, ignore_index, label_smoothing, reduction).backward(grad, lse, saved, want_x, want_w)
+                      ignore_index: int, label_smoothing: float, reduction: str, want_x: bool = True, want_w: bool = True,
+                      grad_bytes: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    dx, dw = _xent_head(x, weight, target, ignore_index, label_smoothing, reduction, grad_bytes).backward(grad, lse, saved, want_x, want_w)
     return _wanted(x, weight, dx, dw, want_x, want_w)
 
 
 @_xent_backward_op.register_fake
-def _(grad, x, weight, target, lse, saved, ignore_index, label_smoothing, reduction, want_x=True, want_w=True):
+def _(grad, x, weight, target, lse, saved, ignore_index, label_smoothing, reduction, want_x=True, want_w=True, grad_bytes=0):
     return _fake_wanted(x, weight, want_x, want_w)
 
 
@@ -330,7 +335,7 @@ def _watch_operator(ctx, x: torch.Tensor, w: torch.Tensor) -> None:
 
 
 def _xent_setup(ctx, inputs, output):
-    x, weight, target, ctx.ignore_index, ctx.label_smoothing, ctx.reduction = inputs
+    x, weight, target, *ctx.options, ctx.grad_bytes = inputs
     _watch_operator(ctx, x, weight)
     ctx.mark_non_differentiable(output[1], output[2])
     ctx.save_for_backward(x, weight, target, output[1], output[2])
@@ -338,8 +343,8 @@ def _xent_setup(ctx, inputs, output):
 
 def _xent_autograd(ctx, grad, _lse, _saved):
     want_x, want_w = ctx.needs_input_grad[:2]
-    dx, dw = torch.ops.aster_b200.linear_cross_entropy_backward(grad, *ctx.saved_tensors, ctx.ignore_index, ctx.label_smoothing, ctx.reduction, want_x, want_w)
-    return dx if want_x else None, dw if want_w else None, None, None, None, None
+    dx, dw = torch.ops.aster_b200.linear_cross_entropy_backward(grad, *ctx.saved_tensors, *ctx.options, want_x, want_w, ctx.grad_bytes)
+    return dx if want_x else None, dw if want_w else None, None, None, None, None, None
 
 
 _xent_op.register_autograd(_xent_autograd, setup_context=_xent_setup)
@@ -347,32 +352,32 @@ _xent_op.register_autograd(_xent_autograd, setup_context=_xent_setup)
 
 @torch.library.custom_op("aster_b200::linear_distillation", mutates_args=())
 def _distill_op(x: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor, temperature: float = 1.0,
-                reduction: str = "mean") -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    head = _distill_head(x, weight, teacher_logits, teacher_ids, temperature, reduction)
+                reduction: str = "mean", grad_bytes: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    head = _distill_head(x, weight, teacher_logits, teacher_ids, temperature, reduction, grad_bytes)
     loss, lse, saved = head.forward()
     return loss.view(teacher_ids.shape[:-1]) if head.per_row else loss, lse, saved
 
 
 @_distill_op.register_fake
-def _(x, weight, teacher_logits, teacher_ids, temperature=1.0, reduction="mean"):
+def _(x, weight, teacher_logits, teacher_ids, temperature=1.0, reduction="mean", grad_bytes=0):
     rows, top = x.numel() // x.shape[-1], teacher_ids.shape[-1]
     return _fake_outputs(x, reduction, teacher_ids.shape[:-1], 256 + _align256(4 * rows) + 2 * _align256(4 * rows * top) if rows else 0)
 
 
 @torch.library.custom_op("aster_b200::linear_distillation_backward", mutates_args=())
 def _distill_backward_op(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, lse: torch.Tensor, saved: torch.Tensor,
-                         temperature: float, reduction: str, want_x: bool = True, want_w: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
-    dx, dw = _distill_head(x, weight, None, teacher_ids, temperature, reduction).backward(grad, lse, saved, want_x, want_w)
+                         temperature: float, reduction: str, want_x: bool = True, want_w: bool = True, grad_bytes: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    dx, dw = _distill_head(x, weight, None, teacher_ids, temperature, reduction, grad_bytes).backward(grad, lse, saved, want_x, want_w)
     return _wanted(x, weight, dx, dw, want_x, want_w)
 
 
 @_distill_backward_op.register_fake
-def _(grad, x, weight, teacher_ids, lse, saved, temperature, reduction, want_x=True, want_w=True):
+def _(grad, x, weight, teacher_ids, lse, saved, temperature, reduction, want_x=True, want_w=True, grad_bytes=0):
     return _fake_wanted(x, weight, want_x, want_w)
 
 
 def _distill_setup(ctx, inputs, output):
-    x, weight, _, teacher_ids, ctx.temperature, ctx.reduction = inputs
+    x, weight, _, teacher_ids, *ctx.options, ctx.grad_bytes = inputs
     _watch_operator(ctx, x, weight)
     ctx.mark_non_differentiable(output[1], output[2])
     ctx.save_for_backward(x, weight, teacher_ids, output[1], output[2])
@@ -380,8 +385,8 @@ def _distill_setup(ctx, inputs, output):
 
 def _distill_autograd(ctx, grad, _lse, _saved):
     want_x, want_w = ctx.needs_input_grad[:2]
-    dx, dw = torch.ops.aster_b200.linear_distillation_backward(grad, *ctx.saved_tensors, ctx.temperature, ctx.reduction, want_x, want_w)
-    return dx if want_x else None, dw if want_w else None, None, None, None, None
+    dx, dw = torch.ops.aster_b200.linear_distillation_backward(grad, *ctx.saved_tensors, *ctx.options, want_x, want_w, ctx.grad_bytes)
+    return dx if want_x else None, dw if want_w else None, None, None, None, None, None
 
 
 _distill_op.register_autograd(_distill_autograd, setup_context=_distill_setup)

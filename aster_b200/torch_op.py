@@ -209,6 +209,12 @@ def quantize_mx_direct(x: torch.Tensor, elem: str = "e2m1") -> tuple[torch.Tenso
     """``x`` ``[M, K]`` (float32, bfloat16 or float16; K a multiple of 32; rows may be strided) to
     block-scaled fp4: packed codes uint8 ``[M, K/2]`` and the packed scales.  A block of 32 that holds
     a NaN or an infinity reads as 32 NaN afterwards."""
+    if torch.compiler.is_compiling():  # a compiler sees the operator, not what is behind it
+        return torch.ops.aster_b200.quantize_mx(x, elem)
+    return _quantize(x, elem)
+
+
+def _quantize(x: torch.Tensor, elem: str) -> tuple[torch.Tensor, torch.Tensor]:
     if elem != "e2m1":
         raise RuntimeError(f"quantize_mx makes e2m1 elements, not {elem!r}")
     if not x.is_cuda:
@@ -228,6 +234,12 @@ def quantize_mx_direct(x: torch.Tensor, elem: str = "e2m1") -> tuple[torch.Tenso
 
 def dequantize_mx_direct(q: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values ``[M, K]`` that packed codes and scales stand for (exact in float32 and bfloat16)."""
+    if torch.compiler.is_compiling():
+        return torch.ops.aster_b200.dequantize_mx(q, scales, out_dtype)
+    return _dequantize(q, scales, out_dtype)
+
+
+def _dequantize(q: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
     _check_mx_operand("q", q, scales)
     if out_dtype not in _MX_VALUE_DTYPES:
         raise RuntimeError(f"unsupported out_dtype {out_dtype}")
@@ -260,6 +272,12 @@ def gemm_mx_nt_direct(a: torch.Tensor, scales_a: torch.Tensor, b: torch.Tensor, 
     them: ``a`` ``[M, K/2]``, ``b`` ``[N, K/2]``, optional float32 ``bias`` ``[N]`` and ReLU, fp32
     accumulation, ``[M, N]`` out.  There is no backward pass: one that reaches the bias is refused.  The first
     call of a shape allocates (its plan lives until :func:`clear_plan_cache`): inside a stream capture it is refused."""
+    if torch.compiler.is_compiling():
+        return torch.ops.aster_b200.gemm_mx_nt(a, scales_a, b, scales_b, bias, relu, out_dtype)
+    return _product(a, scales_a, b, scales_b, bias, relu, out_dtype)
+
+
+def _product(a, scales_a, b, scales_b, bias, relu: bool, out_dtype: torch.dtype) -> torch.Tensor:
     _check_mx_operand("a", a, scales_a)
     _check_mx_operand("b", b, scales_b)
     if a.device != b.device or a.shape[1] != b.shape[1]:
@@ -298,7 +316,7 @@ def _gemm_mx(a, scales_a, b, scales_b, bias, relu, out, stream) -> int:
 
 @torch.library.custom_op("aster_b200::quantize_mx", mutates_args=())
 def quantize_mx(x: torch.Tensor, elem: str = "e2m1") -> tuple[torch.Tensor, torch.Tensor]:
-    return quantize_mx_direct(x, elem)
+    return _quantize(x, elem)
 
 
 @quantize_mx.register_fake
@@ -309,7 +327,7 @@ def _(x, elem="e2m1"):
 
 @torch.library.custom_op("aster_b200::dequantize_mx", mutates_args=())
 def dequantize_mx(q: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    return dequantize_mx_direct(q, scales, out_dtype)
+    return _dequantize(q, scales, out_dtype)
 
 
 @dequantize_mx.register_fake
@@ -320,7 +338,7 @@ def _(q, scales, out_dtype=torch.float32):
 @torch.library.custom_op("aster_b200::gemm_mx_nt", mutates_args=())
 def gemm_mx_nt(a: torch.Tensor, scales_a: torch.Tensor, b: torch.Tensor, scales_b: torch.Tensor, bias: Optional[torch.Tensor] = None,
                relu: bool = False, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    return gemm_mx_nt_direct(a, scales_a, b, scales_b, bias, relu, out_dtype)
+    return _product(a, scales_a, b, scales_b, bias, relu, out_dtype)
 
 
 @gemm_mx_nt.register_fake

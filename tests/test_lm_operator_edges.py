@@ -419,3 +419,41 @@ class TestOperatorsAsTorchKnowsThem:
             x.requires_grad_(frozen is not x), w.requires_grad_(frozen is not w)
             opcheck(ops.linear_cross_entropy.default, (x, w, t, -100, 0.1, "none" if frozen is None else "mean"))
             opcheck(ops.linear_distillation.default, (x, w, logits, ids, 2.0))
+
+    @pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+    def test_functions_inside_a_compiled_program(self, gpu, backend):
+        x, w, t = strided_problem("cuda")
+        x.requires_grad_(), w.requires_grad_()
+        ids, logits = t[:, None].contiguous(), torch.zeros(70, 1, device="cuda")
+        for call in (lambda x, w: hl.linear_cross_entropy(x, w, t, label_smoothing=0.1, grad_bytes=1), lambda x, w: hl.linear_distillation(x, w, logits, ids, reduction="none").sum()):
+            want = call(x, w)
+            loss = torch.compile(call, backend=backend, fullgraph=True)(x, w)
+            assert torch.equal(loss, want)
+            for a, b in zip(torch.autograd.grad(loss, (x, w)), torch.autograd.grad(want, (x, w))):
+                assert torch.equal(a, b)
+
+        def layer(h, v):
+            q, s = top.quantize_mx_direct(h)
+            u, r = top.quantize_mx_direct(v)
+            return top.gemm_mx_nt_direct(q, s, u, r, None, True, torch.bfloat16), top.dequantize_mx_direct(q, s, torch.bfloat16)
+
+        h, v = torch.randn(48, 128, device="cuda").bfloat16(), torch.randn(72, 128, device="cuda").bfloat16()
+        for a, b in zip(torch.compile(layer, backend=backend, fullgraph=True)(h, v), layer(h, v)):
+            assert torch.equal(a, b)
+
+
+class TestOperatorsTakeWhatTheFunctionsTake:
+    def test_limit_of_the_stored_range_on_the_host(self):
+        x, w, t = (v.to("meta") for v in strided_problem("cpu"))
+        x.requires_grad_()
+        ops = torch.ops.aster_b200
+        ops.linear_cross_entropy(x, w, t, -100, 0.0, "mean", 1 << 20)[0].backward()
+        ops.linear_distillation(x, w, torch.zeros(70, 1, device="meta"), t[:, None], 1.0, "mean", 1 << 20)[0].backward()
+
+    @pytest.mark.gpu
+    def test_limit_of_the_stored_range(self, gpu):
+        x, w, t = strided_problem("cuda")
+        x.requires_grad_(), w.requires_grad_()
+        want = torch.autograd.grad(hl.linear_cross_entropy(x, w, t, grad_bytes=1), (x, w))
+        got = torch.autograd.grad(torch.ops.aster_b200.linear_cross_entropy(x, w, t, grad_bytes=1)[0], (x, w))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
