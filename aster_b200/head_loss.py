@@ -23,10 +23,9 @@ import weakref
 from typing import Optional, Sequence
 
 import torch
-from torch.autograd import forward_ad
 
 from . import _native as nat
-from .torch_op import _call, _raw_stream
+from .torch_op import _call, _raw_stream, has_tangent
 
 _DTYPES = {torch.bfloat16: nat.BF16, torch.float16: nat.F16}
 _TEACHER_DTYPES = {torch.float32: nat.F32, torch.bfloat16: nat.BF16, torch.float16: nat.F16}
@@ -47,7 +46,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _check(name: str, x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, reduction: str) -> None:
-    if forward_ad.unpack_dual(x).tangent is not None or forward_ad.unpack_dual(w).tangent is not None:
+    if has_tangent(x, w):
         raise RuntimeError(f"aster_b200::{name} has no forward-mode derivative: x and weight must not carry a tangent")
     for what, t in (("x", x), ("weight", w), ("labels", labels)):
         if not t.is_cuda:
@@ -92,12 +91,17 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def _saw(*tensors: torch.Tensor) -> list:
+    """What the tensors of a pass have to have in common with those of the other one."""
+    return [(t.shape, t.dtype, t.device) for t in tensors]
+
+
 class _Head:
     """One call's tensors as the C ABI wants them, and its description."""
 
     def __init__(self, x, w, labels, reduction, *, kind, ignore_index=0, label_smoothing=0.0, temperature=1.0, teacher=None, grad_bytes=0):
         self.x, self.w, self.labels, self.teacher = _rows(x), _rows(w), labels.contiguous(), teacher
-        self.device, self.shapes = x.device, (self.x.shape, self.w.shape, self.labels.shape)
+        self.device, self.saw = x.device, _saw(self.x, self.w, self.labels)
         self.desc = d = _desc(self.x, self.w, labels, reduction)
         d.kind, d.ignore_index, d.label_smoothing, d.temperature = kind, ignore_index, label_smoothing, temperature
         d.grad_bytes = grad_bytes
@@ -108,7 +112,7 @@ class _Head:
     def without_tensors(self) -> "_Head":
         """The description alone, for the time until the backward pass brings the tensors again."""
         h = _Head.__new__(_Head)
-        h.desc, h.per_row, h.device, h.shapes = self.desc, self.per_row, self.device, self.shapes
+        h.desc, h.per_row, h.device, h.saw = self.desc, self.per_row, self.device, self.saw
         return h
 
     def with_tensors(self, x, w, labels) -> "_Head":
@@ -118,14 +122,13 @@ class _Head:
         h.x, h.w, h.labels, h.teacher = _rows(x), _rows(w), labels.contiguous(), None
         x, w, labels = h.x, h.w, h.labels
         d = self.desc
-        if (x.shape, w.shape, labels.shape) != self.shapes or _DTYPES.get(x.dtype) != d.dtype or w.dtype != x.dtype or _INDEX_BITS.get(labels.dtype) != d.index_bits:
-            raise RuntimeError("the saved tensors came back with another shape or dtype than the forward pass had")
-        if not x.device == w.device == labels.device == self.device:
-            raise RuntimeError(f"the saved tensors came back on {x.device}, {w.device} and {labels.device}, not on {self.device}")
-        strides = x.stride(0) if d.tokens > 1 else d.hidden, w.stride(0) if d.vocab > 1 else d.hidden
-        if strides != (d.x_stride, d.w_stride):
+        saw = _saw(x, w, labels)
+        if saw != self.saw:
+            raise RuntimeError(f"the saved tensors came back as {saw}; the forward pass had {self.saw}")
+        x_stride, w_stride = x.stride(0) if d.tokens > 1 else d.hidden, w.stride(0) if d.vocab > 1 else d.hidden
+        if x_stride != d.x_stride or w_stride != d.w_stride:
             h.desc = nat.HeadDesc.from_buffer_copy(d)
-            h.desc.x_stride, h.desc.w_stride = strides
+            h.desc.x_stride, h.desc.w_stride = x_stride, w_stride
         return h
 
     def forward(self):

@@ -198,6 +198,12 @@ def _check_mx_operand(name: str, q: torch.Tensor, scales: torch.Tensor) -> None:
         raise RuntimeError(f"{name}'s scales must be the {want} packed bytes on {q.device} that quantize_mx returns, got {tuple(scales.shape)} on {scales.device}")
 
 
+def has_tangent(*tensors: torch.Tensor) -> bool:
+    """Does one of them carry a forward-mode tangent?  (Outside of a dual level, where none can, asking each of
+    them would cost 0.7 us.)"""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """Contiguous and 16-byte aligned (a view can start anywhere)."""
     if not t.is_contiguous():
@@ -287,7 +293,7 @@ def _product(a, scales_a, b, scales_b, bias, relu: bool, out_dtype: torch.dtype)
     M, N, K = a.shape[0], b.shape[0], 2 * a.shape[1]
     if bias is not None and (bias.dtype != torch.float32 or bias.device != a.device or bias.numel() != N):
         raise RuntimeError(f"bias must be {N} float32 values on {a.device}")
-    if bias is not None and forward_ad.unpack_dual(bias).tangent is not None:
+    if bias is not None and has_tangent(bias):
         raise RuntimeError("aster_b200::gemm_mx_nt has no forward-mode derivative: bias must not carry a tangent")
     a, scales_a, b, scales_b = _aligned(a), _aligned(scales_a), _aligned(b), _aligned(scales_b)
     bias = None if bias is None else bias.contiguous()
