@@ -352,7 +352,10 @@ typedef struct b200_head_desc {
   int32_t dtype_teacher;       /* distillation: B200_F32 | B200_BF16 | B200_F16                 */
   float label_smoothing;       /* cross entropy: [0, 1)                                         */
   float temperature;           /* distillation: 2^-60 .. 2^60                                   */
-  int64_t grad_bytes;          /* limit of the stored range of dL/dz; 0 = 256 MiB               */
+  int64_t grad_bytes;          /* limit of the stored range of dL/dz; 0 = 256 MiB; never below
+                                * 256 columns, i.e. 512 * tokens bytes.  fp32 parts of grad_x
+                                * (grad_splits * tokens * hidden, with more than one range or part)
+                                * and of grad_w (at most 256 MiB) come on top                   */
   int32_t wait_limit_ms;       /* limit of the device-side waits; 0 = 2000                      */
   int32_t reserved;
 } b200_head_desc;
