@@ -22,7 +22,7 @@ Precision.  Products, softmax sums and losses are fp32, but not every step round
 * ``dL/dz`` is rounded once to the operands' 16 bits before both gradient products, after division by the
   largest row factor: with one label per row the gradients are as near as their own rounding, with a teacher's
   many entries about 1.4 times as far (bf16 0.0024 against 0.0017).  With "none" in float16 a row whose factor
-  is below 1e-8 of the largest loses digits of its gradient, below 1e-11 all of them;
+  is below 1e-8 of the largest loses digits of its gradient, below 3e-12 all of them;
 * the gradients are products: an ignored row of ``x`` that holds NaN or infinity reaches ``dL/dw`` (0 * NaN),
   and one of ``w`` reaches ``dL/dx``, as in the plain program.
 

@@ -330,7 +330,7 @@ int b200_dequantize_mx(const void* q, const void* scales_packed, int32_t dtype_q
  * the sum of exp(z / T)) and `saved` are what the backward pass needs again, beside the same inputs.
  * grad_loss: [tokens] fp32 for NONE, else one fp32.  grad_x [tokens][hidden] and grad_w [vocab][hidden] are
  * 16-bit like the operands, contiguous; either may be NULL (not wanted).  Sums over hidden, tokens and the
- * vocabulary are fp32; the gradient of z, divided by its largest row factor, is rounded to 16 bits once
+ * vocabulary are fp32 (the tensor core's accumulator truncates); the gradient of z, divided by its largest row factor, is rounded to 16 bits once
  * before the last two products; probabilities below 2^-126 count as 0.  Every result is the same
  * from run to run.
  * hidden: a multiple of 8, below 2^31; x, w, grad_x, grad_w, saved and the workspaces 16-byte aligned, rows of x and w
