@@ -258,8 +258,8 @@ def _dequantize(q: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype) -
 
 class _NoGradient(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, out, bias):
-        return out.view_as(out)
+    def forward(ctx, bias, made):
+        return made.pop()  # not an input: the result is no view of one and may be changed in place
 
     @staticmethod
     def backward(ctx, grad):
@@ -269,7 +269,7 @@ class _NoGradient(torch.autograd.Function):
 def _without_gradient(out: torch.Tensor, bias: torch.Tensor) -> torch.Tensor:
     """``out`` as part of ``bias``'s graph: a backward pass that reaches it is refused, as the dispatcher's form
     does, where a result without a graph would leave the bias out of it silently."""
-    return _NoGradient.apply(out, bias)
+    return _NoGradient.apply(bias, [out])
 
 
 def gemm_mx_nt_direct(a: torch.Tensor, scales_a: torch.Tensor, b: torch.Tensor, scales_b: torch.Tensor, bias: Optional[torch.Tensor] = None,

@@ -370,6 +370,8 @@ class TestProductHasNoBackward:
         assert c.requires_grad and torch.equal(c.detach(), out)
         with pytest.raises(RuntimeError, match="no backward pass"):
             c.sum().backward()
+        top._without_gradient(out, bias).add_(1.0)  # in place, like any fresh result
+        assert bool((out == 1).all())
 
     @pytest.mark.gpu
     @pytest.mark.parametrize("form", ["direct", "operator"])
