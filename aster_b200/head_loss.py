@@ -18,7 +18,7 @@ is used, there is no CPU path and no fallback.
 Precision.  Products, softmax sums and losses are fp32, but not every step rounds as a plain fp32 program's:
 
 * the tensor core's accumulator truncates: logits come out up to (hidden / 16 + 1) * 2^-23 * |x| . |w| off
-  (9e-6 rms at hidden = 4096, losses 1.5e-6 relative), and exponentials are the hardware's (2 ulp);
+  (9e-6 rms at hidden = 4096, losses 1.5e-6 relative), and exponentials are the hardware's (2 ulp, 0 below 2^-126);
 * ``dL/dz`` is rounded once to the operands' 16 bits before both gradient products, after division by the
   largest row factor: with one label per row the gradients are as near as their own rounding, with a teacher's
   many entries about 1.4 times as far (bf16 0.0024 against 0.0017).  With "none" in float16 a row whose factor

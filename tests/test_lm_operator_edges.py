@@ -459,3 +459,51 @@ class TestOperatorsTakeWhatTheFunctionsTake:
         want = torch.autograd.grad(hl.linear_cross_entropy(x, w, t, grad_bytes=1), (x, w))
         got = torch.autograd.grad(torch.ops.aster_b200.linear_cross_entropy(x, w, t, grad_bytes=1)[0], (x, w))
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+class TestTwoAtOnce:
+    """Two captured graphs of the same shapes, replayed on two streams at the same time, and eager calls beside them."""
+
+    @staticmethod
+    def replay(graphs, outs, wants, beside):
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for _ in range(20):
+            torch.cuda.synchronize()
+            for stream, graph in zip(streams, graphs):
+                with torch.cuda.stream(stream):
+                    for _ in range(5):
+                        graph.replay()
+            eager = beside()
+            torch.cuda.synchronize()
+            for out, want in zip(outs + [eager], wants + [wants[0]]):
+                assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+    @pytest.mark.parametrize("shape", [(16, 1024, 8192), (300, 520, 1056)])  # K cut between CTAs, pair tiles
+    def test_products_of_one_plan(self, gpu, shape):
+        M, N, K = shape
+        operands = [top.quantize_mx_direct(torch.randn(M, K, device="cuda")) + top.quantize_mx_direct(torch.randn(N, K, device="cuda")) for _ in range(2)]
+        wants = [[top.gemm_mx_nt_direct(*o)] for o in operands]
+        graphs, outs = [torch.cuda.CUDAGraph() for _ in operands], []
+        for graph, o in zip(graphs, operands):
+            with torch.cuda.graph(graph):
+                outs.append([top.gemm_mx_nt_direct(*o)])
+        self.replay(graphs, outs, wants, lambda: [top.gemm_mx_nt_direct(*operands[0])])
+
+    @pytest.mark.parametrize("distill", [False, True])
+    def test_training_steps(self, gpu, distill):
+        def step(x, w, t):
+            loss = hl.linear_distillation(x, w, torch.zeros(70, 1, device="cuda"), t[:, None]) if distill else hl.linear_cross_entropy(x, w, t, label_smoothing=0.1)
+            return [loss.detach(), *torch.autograd.grad(loss, (x, w))]
+
+        problems = []
+        for seed in (3, 4):
+            x, w, t = strided_problem("cuda", V=3001, seed=seed)
+            problems.append((x.requires_grad_(), w.requires_grad_(), t))
+        wants = [step(*p) for p in problems]
+        graphs, outs = [torch.cuda.CUDAGraph() for _ in problems], []
+        for graph, p in zip(graphs, problems):
+            with torch.cuda.graph(graph):
+                outs.append(step(*p))
+        self.replay(graphs, outs, wants, lambda: step(*problems[0]))
+        assert hl.head_loss_status() == [0, 0, 0, 0]
